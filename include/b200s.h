@@ -35,7 +35,8 @@ typedef enum b200s_status {
   B200S_ERR_NO_DEVICE = -10,    /* no sm_100 device is current */
   B200S_ERR_DEVICE_TIMEOUT = -11, /* a kernel gave up on a bounded wait (read by b200s_device_status) */
   B200S_ERR_TUNER_IO = -12,
-  B200S_ERR_TOO_LARGE = -13     /* problem exceeds the fixed capacity of a no-allocation entry point */
+  B200S_ERR_TOO_LARGE = -13,    /* problem exceeds the fixed capacity of a no-allocation entry point */
+  B200S_ERR_OVERLAP = -14       /* tensors of a list overlap where one of them is written */
 } b200s_status;
 
 typedef enum b200s_dtype { B200S_BF16 = 0, B200S_FP16 = 1, B200S_FP32 = 2 } b200s_dtype;
@@ -334,6 +335,135 @@ int b200s_set_product_sms(int n);
 int b200s_set_sender_sms(int n);
 int b200s_push_panel(const void* src_device, void* const* dst_list, int n_dst, void* mc_dst, size_t bytes,
                      int max_blocks, void* stream);
+
+/*
+ * ---- Operators of a training step beside its matrix products ------------------------------------
+ *
+ * The parts of a transformer's step that surround the products above: layer norm, the epilogue of a
+ * linear layer, the token loss, the gradient norm. Matrices of rows: element (r, c) of a matrix at X
+ * with leading dimension ld (in ELEMENTS) is X[r * ld + c]; pointers need the alignment of their
+ * element type only (16-byte aligned rows are faster). Input rows may repeat or overlap (ld >= 0),
+ * output rows may not (ld >= the row's length). rows = 0 is allowed and launches nothing but what a
+ * gradient of zero rows needs. Sums and statistics are fp32 (fp64 where stated); every result is
+ * rounded once, to the type it is stored in, and does not depend on timing: the same call gives the
+ * same bits. All are asynchronous on `stream` and may be captured into a graph after a first call
+ * outside capture. The reference's model code leaves these steps to torch (its nn.LayerNorm /
+ * F.cross_entropy / F.gelu calls); there is no counterpart among its kernels.
+ */
+
+/*
+ * y = (x - mean) * rstd * weight + bias over rows of d elements, rstd = 1/sqrt(var + eps).
+ * dtype: type of x and y. weight and bias (each may be NULL: 1 and 0) hold d elements of param_dtype,
+ * which is dtype or B200S_FP32. mean and rstd (both or neither NULL) receive `rows` fp32 values each,
+ * which the backward pass takes.
+ */
+int b200s_layer_norm(int64_t rows, int64_t d, int dtype, int param_dtype, float eps, const void* x_device,
+                     int64_t ldx, const void* weight_device, const void* bias_device, void* y_device, int64_t ldy,
+                     float* mean_device, float* rstd_device, void* stream);
+
+/*
+ * Gradients of b200s_layer_norm: dx (may be NULL) of type dtype, dweight and dbias (each may be NULL)
+ * of d elements of param_dtype. The sums over rows go through fp32 partial sums in `workspace` (16-byte
+ * aligned, b200s_layer_norm_backward_workspace bytes; may be NULL when neither dweight nor dbias is
+ * wanted) and are added in a fixed order.
+ */
+int b200s_layer_norm_backward_workspace(int64_t rows, int64_t d, size_t* bytes_out);
+int b200s_layer_norm_backward(int64_t rows, int64_t d, int dtype, int param_dtype, const void* x_device, int64_t ldx,
+                              const void* dy_device, int64_t lddy, const void* weight_device,
+                              const float* mean_device, const float* rstd_device, void* dx_device, int64_t lddx,
+                              void* dweight_device, void* dbias_device, void* workspace_device,
+                              size_t workspace_bytes, void* stream);
+
+/* Activation of a product's epilogue. */
+typedef enum b200s_activation {
+  B200S_ACT_NONE = 0,
+  B200S_ACT_RELU = 1,
+  B200S_ACT_RELU2 = 2,    /* max(z, 0)^2 */
+  B200S_ACT_SILU = 3,     /* z sigmoid(z) */
+  B200S_ACT_GELU = 4,     /* z Phi(z), Phi the normal distribution function */
+  B200S_ACT_GELU_TANH = 5 /* its tanh form, 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+} b200s_activation;
+
+typedef struct b200s_epilogue {
+  int32_t activation;     /* b200s_activation */
+  int32_t reserved;       /* 0 */
+  const void* bias;       /* device, N elements of out_dtype, or NULL */
+  const void* residual;   /* device, M x N of out_dtype, or NULL */
+  int64_t ld_residual;
+  void* preact;           /* device, M x N of out_dtype, or NULL: receives z for b200s_epilogue_backward */
+  int64_t ld_preact;
+} b200s_epilogue;
+
+/*
+ * z = A . B + bias, C = act(z) + residual: a linear layer with its epilogue in one call. Everything
+ * after the product happens in fp32 and C is rounded once; z is also stored (rounded) when `preact` is
+ * given. The product is p's (any algorithm and depth; beta 0, batch 1). residual may be C itself (the
+ * same address and leading dimension). Scratch: b200s_matmul_epilogue_workspace bytes (which looks at
+ * p and e->activation only for validation), 256-byte aligned.
+ */
+int b200s_matmul_epilogue_workspace(const b200s_problem* p, const b200s_epilogue* e, size_t* bytes_out);
+int b200s_matmul_epilogue(const b200s_problem* p, const b200s_epilogue* e, const void* A_device, const void* B_device,
+                          void* C_device, void* workspace_device, size_t workspace_bytes, void* stream);
+
+/*
+ * The elementwise part of its backward pass: dz = dy * act'(z) (M x N of dtype; may be NULL) and
+ * dbias = column sums of dz before its rounding (N elements of dtype; may be NULL). `preact` is the z
+ * stored by the forward call (ignored for B200S_ACT_NONE). The gradients of A and B are products of dz
+ * (b200s_matmul), that of the residual is dy itself.
+ */
+int b200s_epilogue_backward_workspace(int64_t M, int64_t N, size_t* bytes_out);
+int b200s_epilogue_backward(int64_t M, int64_t N, int dtype, int activation, const void* preact_device, int64_t ldz,
+                            const void* dy_device, int64_t lddy, void* dz_device, int64_t lddz, void* dbias_device,
+                            void* workspace_device, size_t workspace_bytes, void* stream);
+
+/*
+ * Log probability of one given token per row of logits, the row's log-sum-exp, the entropy of its
+ * distribution and its top_k (0..64) most likely tokens with their log probabilities; all outputs but
+ * token ids are fp32. lse, entropy may be NULL; the top outputs hold top_k values per row, best first,
+ * ties in favour of the lower id. Only the first `vocab` columns of a row count (the rest is padding).
+ * A target equal to ignore_index gives log probability 0; another one outside [0, vocab) gives NaN.
+ * -inf logits are tokens of probability zero; a row of nothing else has lse and logprob -inf, entropy 0.
+ */
+int b200s_token_logprobs(int64_t rows, int64_t vocab, int dtype, const void* logits_device, int64_t ld,
+                         const int64_t* targets_device, int64_t ignore_index, float* logprob_device,
+                         float* lse_device, float* entropy_device, int top_k, int64_t* top_ids_device,
+                         float* top_logprobs_device, void* stream);
+
+/*
+ * dlogits (rows x width of dtype, columns from vocab on zero) from the gradients of the log
+ * probabilities and of the entropies (each may be NULL: zero), with lse and entropy as the forward call
+ * wrote them (entropy is needed with dentropy only). Rows that were ignored and have no entropy gradient,
+ * and rows without a finite logit, get zeros. dlogits may be the logits themselves (same ld).
+ */
+int b200s_token_logprobs_backward(int64_t rows, int64_t vocab, int64_t width, int dtype, const void* logits_device,
+                                  int64_t ld, const int64_t* targets_device, int64_t ignore_index,
+                                  const float* lse_device, const float* entropy_device, const float* dlogprob_device,
+                                  const float* dentropy_device, void* dlogits_device, int64_t ldd, void* stream);
+
+/* One dense tensor of a list: numel elements at src; dst, where a call writes, may be src itself. */
+typedef struct b200s_tensor {
+  const void* src;
+  void* dst;
+  int64_t numel;
+  int32_t dtype;      /* b200s_dtype of src */
+  int32_t dst_dtype;  /* b200s_dtype of dst */
+} b200s_tensor;
+
+#define B200S_NORM_PARTS 592
+
+/*
+ * Global gradient norm and clipping. `list` is a host array of `count` tensors (copied into the launches,
+ * so it may go away and a captured graph keeps it). b200s_grad_sumsq writes the sum of squares of all
+ * elements as B200S_NORM_PARTS fp64 partial sums; b200s_grad_norm adds n_parts of them and writes the
+ * square root (fp32). b200s_grad_clip does the same and sets dst = src * min(1, max_norm / (norm + 1e-6))
+ * for every tensor; tensors with dst == src are not touched when nothing is to be clipped. Between the two
+ * a caller may add the sums of other ranks (add the parts up, reduce, pass n_parts = 1). A dst that
+ * overlaps another tensor of the list (the same tensor twice, say) is refused with B200S_ERR_OVERLAP.
+ */
+int b200s_grad_sumsq(const b200s_tensor* list, int64_t count, double* parts_device, void* stream);
+int b200s_grad_norm(const double* parts_device, int n_parts, float* norm_device, void* stream);
+int b200s_grad_clip(const b200s_tensor* list, int64_t count, const double* parts_device, int n_parts, float max_norm,
+                    float* norm_device, void* stream);
 
 #ifdef __cplusplus
 }

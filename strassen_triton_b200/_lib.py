@@ -33,6 +33,11 @@ ERR_NO_DEVICE = -10
 ERR_DEVICE_TIMEOUT = -11
 ERR_TUNER_IO = -12
 ERR_TOO_LARGE = -13
+ERR_OVERLAP = -14
+
+ACT_NONE, ACT_RELU, ACT_RELU2, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3, 4, 5
+NORM_PARTS = 592
+MAX_TOP_K = 64
 
 
 class Problem(ctypes.Structure):
@@ -51,6 +56,25 @@ class Problem(ctypes.Structure):
     ]
 
 
+class Epilogue(ctypes.Structure):
+    """Mirror of ``struct b200s_epilogue``."""
+
+    _fields_ = [
+        ("activation", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("ld_residual", ctypes.c_int64),
+        ("preact", ctypes.c_void_p), ("ld_preact", ctypes.c_int64),
+    ]
+
+
+class TensorEntry(ctypes.Structure):
+    """Mirror of ``struct b200s_tensor``."""
+
+    _fields_ = [
+        ("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("numel", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("dst_dtype", ctypes.c_int32),
+    ]
+
+
 class B200SError(RuntimeError):
     """A libb200s.so call returned a negative status."""
 
@@ -61,6 +85,7 @@ class B200SError(RuntimeError):
 
 # name -> (restype, argtypes); every symbol include/b200s.h declares.
 _P = ctypes.POINTER
+_PTR, _I64, _INT, _F32, _SIZE = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
 SIGNATURES = {
     "b200s_version": (ctypes.c_int, []),
     "b200s_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -106,6 +131,20 @@ SIGNATURES = {
     "b200s_push_panel": (ctypes.c_int, [ctypes.c_void_p, _P(ctypes.c_void_p), ctypes.c_int, ctypes.c_void_p,
                                         ctypes.c_size_t, ctypes.c_int, ctypes.c_void_p]),
     "b200s_combine": (ctypes.c_int, [_P(Problem), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "b200s_layer_norm": (_INT, [_I64, _I64, _INT, _INT, _F32, _PTR, _I64, _PTR, _PTR, _PTR, _I64, _PTR, _PTR, _PTR]),
+    "b200s_layer_norm_backward_workspace": (_INT, [_I64, _I64, _P(_SIZE)]),
+    "b200s_layer_norm_backward": (_INT, [_I64, _I64, _INT, _INT, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _PTR, _I64,
+                                         _PTR, _PTR, _PTR, _SIZE, _PTR]),
+    "b200s_matmul_epilogue_workspace": (_INT, [_P(Problem), _P(Epilogue), _P(_SIZE)]),
+    "b200s_matmul_epilogue": (_INT, [_P(Problem), _P(Epilogue), _PTR, _PTR, _PTR, _PTR, _SIZE, _PTR]),
+    "b200s_epilogue_backward_workspace": (_INT, [_I64, _I64, _P(_SIZE)]),
+    "b200s_epilogue_backward": (_INT, [_I64, _I64, _INT, _INT, _PTR, _I64, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _SIZE, _PTR]),
+    "b200s_token_logprobs": (_INT, [_I64, _I64, _INT, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _INT, _PTR, _PTR, _PTR]),
+    "b200s_token_logprobs_backward": (_INT, [_I64, _I64, _I64, _INT, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _PTR, _PTR,
+                                             _I64, _PTR]),
+    "b200s_grad_sumsq": (_INT, [_PTR, _I64, _PTR, _PTR]),
+    "b200s_grad_norm": (_INT, [_PTR, _INT, _PTR, _PTR]),
+    "b200s_grad_clip": (_INT, [_PTR, _I64, _PTR, _INT, _F32, _PTR, _PTR]),
 }
 
 _lib = None
@@ -147,6 +186,6 @@ def check(status: int) -> None:
     text = status_string(status)
     if status == ERR_CUDA:
         text += ": " + load().b200s_last_cuda_error().decode()
-    if status in (ERR_BAD_SHAPE, ERR_BAD_DEPTH):
+    if status in (ERR_BAD_SHAPE, ERR_BAD_DEPTH, ERR_OVERLAP):
         raise ValueError(f"b200s status {status}: {text}")
     raise B200SError(status, text)

@@ -569,6 +569,7 @@ const char* b200s_status_string(int status) {
     case B200S_ERR_NO_DEVICE: return "current device is not an sm_100 GPU";
     case B200S_ERR_DEVICE_TIMEOUT: return "a kernel gave up on a bounded wait";
     case B200S_ERR_TUNER_IO: return "tuner table file could not be read or written";
+    case B200S_ERR_OVERLAP: return "tensors of the list overlap where one of them is written";
     case B200S_ERR_TOO_LARGE: return "problem exceeds the fixed capacity of this entry point";
   }
   return "unknown status";

@@ -1,0 +1,69 @@
+// Activations of the linear layer's epilogue and their derivatives, in fp32.
+//
+//   relu2(z) = max(z, 0)^2            silu(z) = z sigmoid(z)
+//   gelu(z) = z Phi(z), Phi the normal distribution function
+//   gelu_tanh(z) = z sigmoid(2 c (z + 0.044715 z^3)), c = sqrt(2 / pi): (1 + tanh a) / 2 = sigmoid(2a)
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "../../include/b200s.h"
+
+namespace b200s {
+namespace epi {
+
+constexpr float kTanhC = 0.7978845608028654f;    // sqrt(2 / pi)
+constexpr float kTanhA = 0.044715f;
+constexpr float kPdf0 = 0.3989422804014327f;     // 1 / sqrt(2 pi)
+
+template <int ACT>
+__device__ __forceinline__ float act(float z) {
+  if constexpr (ACT == B200S_ACT_RELU) return z < 0.f ? 0.f : z;       // NaN stays NaN
+  if constexpr (ACT == B200S_ACT_RELU2) return z < 0.f ? 0.f : z * z;
+  if constexpr (ACT == B200S_ACT_SILU) return z * (1.f / (1.f + __expf(-z)));
+  if constexpr (ACT == B200S_ACT_GELU) return z * normcdff(z);
+  if constexpr (ACT == B200S_ACT_GELU_TANH) return z * (1.f / (1.f + __expf(-2.f * kTanhC * fmaf(kTanhA * z, z * z, z))));
+  return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float dact(float z) {
+  if constexpr (ACT == B200S_ACT_RELU) return z > 0.f ? 1.f : (z == z ? 0.f : z);
+  if constexpr (ACT == B200S_ACT_RELU2) return z > 0.f ? 2.f * z : (z == z ? 0.f : z);
+  if constexpr (ACT == B200S_ACT_SILU) {
+    const float t = fminf(fmaxf(z, -80.f), 80.f);                      // beyond, the limits 0 and 1 hold to the last bit
+    const float s = 1.f / (1.f + __expf(-t));
+    return (z == z) ? s * fmaf(t, 1.f - s, 1.f) : z;
+  }
+  if constexpr (ACT == B200S_ACT_GELU) {
+    const float t = fminf(fmaxf(z, -20.f), 20.f);
+    return (z == z) ? fmaf(t * kPdf0, __expf(-0.5f * t * t), normcdff(t)) : z;
+  }
+  if constexpr (ACT == B200S_ACT_GELU_TANH) {
+    const float t = fminf(fmaxf(z, -20.f), 20.f);
+    const float s = 1.f / (1.f + __expf(-2.f * kTanhC * fmaf(kTanhA * t, t * t, t)));
+    return (z == z) ? fmaf(t * s * (1.f - s), 2.f * kTanhC * fmaf(3.f * kTanhA * t, t, 1.f), s) : z;
+  }
+  return 1.f;
+}
+
+// f(std::integral_constant<int, ACT>) for the activation known at run time.
+template <int N>
+struct Act {
+  static constexpr int value = N;
+};
+template <typename F>
+__host__ int by_activation(int a, F&& f) {
+  switch (a) {
+    case B200S_ACT_NONE: return f(Act<B200S_ACT_NONE>{});
+    case B200S_ACT_RELU: return f(Act<B200S_ACT_RELU>{});
+    case B200S_ACT_RELU2: return f(Act<B200S_ACT_RELU2>{});
+    case B200S_ACT_SILU: return f(Act<B200S_ACT_SILU>{});
+    case B200S_ACT_GELU: return f(Act<B200S_ACT_GELU>{});
+    case B200S_ACT_GELU_TANH: return f(Act<B200S_ACT_GELU_TANH>{});
+  }
+  return B200S_ERR_BAD_ALGO;
+}
+
+}  // namespace epi
+}  // namespace b200s

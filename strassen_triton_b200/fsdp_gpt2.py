@@ -10,6 +10,11 @@ reduce-scatter.
 
     torchrun --nproc-per-node 8 -m strassen_triton_b200.fsdp_gpt2 --steps 10
     python -m strassen_triton_b200.fsdp_gpt2 --layers 2 --steps 3          # one GPU
+    python -m strassen_triton_b200.fsdp_gpt2 --fused --clip 1.0            # norms, epilogues, loss and clipping too
+
+With ``fused`` the step around the products also runs on the library: layer norms, GELU and the residual
+additions in the products' epilogues, the loss from the bf16 logits (over the 50257 real columns), and
+with ``clip`` the gradient norm and clipping. Without it those parts are torch's.
 
 The reference's training configuration at GPT-2-124M size: 12 layers, d = 768, 12 heads, vocab 50257 (padded to 50304 rows so that every
 matrix row is a whole number of 16-byte vectors), sequence 1024, 8 sequences per GPU.
@@ -30,7 +35,10 @@ from torch.distributed.fsdp import FullyShardedDataParallel as FSDP
 from torch.distributed.fsdp import MixedPrecision
 from torch.distributed.fsdp.wrap import transformer_auto_wrap_policy
 
+from .grads import clip_grad_norm_
 from .linear import LinearStrassen
+from .loss import cross_entropy
+from .norm import LayerNorm
 
 VOCAB = 50257
 VOCAB_PADDED = 50304
@@ -44,32 +52,43 @@ def _linear_factory(depth, device, plain: bool):
 
 
 class Block(nn.Module):
-    def __init__(self, d: int, heads: int, depth, device, plain: bool = False):
+    def __init__(self, d: int, heads: int, depth, device, plain: bool = False, fused: bool = False):
         super().__init__()
+        if plain and fused:
+            raise ValueError("plain layers have no fused form")
         mk = _linear_factory(depth, device, plain)
-        self.heads = heads
-        self.ln1 = nn.LayerNorm(d, device=device)
-        self.ln2 = nn.LayerNorm(d, device=device)
+        norm = LayerNorm if fused else nn.LayerNorm
+        self.heads, self.fused = heads, fused
+        self.ln1 = norm(d, device=device)
+        self.ln2 = norm(d, device=device)
         self.qkv = mk(d, 3 * d)       # X[8192,768] . W[768,2304]
         self.proj = mk(d, d)
         self.fc = mk(d, 4 * d)        # X[8192,768] . W[768,3072]
         self.out = mk(4 * d, d)       # X[8192,3072] . W[3072,768]
+        if fused:
+            self.fc.activation = "gelu"
 
     def forward(self, x):
         b, t, d = x.shape
         q, k, v = self.qkv(self.ln1(x)).view(b, t, 3, self.heads, d // self.heads).permute(2, 0, 3, 1, 4)
         a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
-        x = x + self.proj(a.transpose(1, 2).reshape(b, t, d))
+        a = a.transpose(1, 2).reshape(b, t, d)
+        if self.fused:
+            x = self.proj(a, residual=x)
+            return self.out(self.fc(self.ln2(x)), residual=x)
+        x = x + self.proj(a)
         return x + self.out(F.gelu(self.fc(self.ln2(x))))
 
 
 class GPT(nn.Module):
-    def __init__(self, layers=12, d=768, heads=12, seq=1024, depth=None, device="cuda", plain: bool = False):
+    def __init__(self, layers=12, d=768, heads=12, seq=1024, depth=None, device="cuda", plain: bool = False,
+                 fused: bool = False):
         super().__init__()
+        self.fused = fused
         self.wte = nn.Embedding(VOCAB_PADDED, d, device=device)
         self.wpe = nn.Embedding(seq, d, device=device)
-        self.blocks = nn.ModuleList(Block(d, heads, depth, device, plain) for _ in range(layers))
-        self.ln_f = nn.LayerNorm(d, device=device)
+        self.blocks = nn.ModuleList(Block(d, heads, depth, device, plain, fused) for _ in range(layers))
+        self.ln_f = (LayerNorm if fused else nn.LayerNorm)(d, device=device)
         self.lm_head = _linear_factory(depth, device, plain)(d, VOCAB_PADDED)
         for m in self.modules():
             if isinstance(m, (nn.Linear, nn.Embedding)):
@@ -81,11 +100,13 @@ class GPT(nn.Module):
         for blk in self.blocks:
             x = blk(x)
         logits = self.lm_head(self.ln_f(x))
+        if self.fused:
+            return cross_entropy(logits, targets, vocab=VOCAB)
         return F.cross_entropy(logits.float().view(-1, logits.shape[-1]), targets.reshape(-1))
 
 
-def build(layers, seq, depth, device, world, plain: bool = False, state=None):
-    model = GPT(layers=layers, seq=seq, depth=depth, device=device, plain=plain)
+def build(layers, seq, depth, device, world, plain: bool = False, state=None, fused: bool = False):
+    model = GPT(layers=layers, seq=seq, depth=depth, device=device, plain=plain, fused=fused)
     if state is not None:
         model.load_state_dict(state)
     if world == 0:
@@ -96,8 +117,10 @@ def build(layers, seq, depth, device, world, plain: bool = False, state=None):
                 device_id=torch.cuda.current_device(), sync_module_states=world > 1)
 
 
-def train_steps(model, steps, batch, seq, rank, lr=3e-4):
-    """Runs `steps` optimizer steps on random tokens; returns the list of losses."""
+def train_steps(model, steps, batch, seq, rank, lr=3e-4, clip=0.0):
+    """Runs `steps` optimizer steps on random tokens; returns the list of losses. ``clip`` > 0 clips the
+    gradients to that norm (over the shards of all ranks when the model is wrapped)."""
+    group = dist.group.WORLD if clip and isinstance(model, FSDP) and dist.get_world_size() > 1 else None
     opt = torch.optim.AdamW(model.parameters(), lr=lr, weight_decay=0.0)
     g = torch.Generator(device="cuda").manual_seed(rank)
     losses = []
@@ -105,6 +128,8 @@ def train_steps(model, steps, batch, seq, rank, lr=3e-4):
         ids = torch.randint(0, VOCAB, (batch, seq + 1), generator=g, device="cuda")
         loss = model(ids[:, :-1], ids[:, 1:])
         loss.backward()
+        if clip:
+            clip_grad_norm_(model.parameters(), clip, group=group)
         opt.step()
         opt.zero_grad(set_to_none=True)
         losses.append(loss.item())
@@ -156,6 +181,8 @@ def main():
     ap.add_argument("--batch", type=int, default=8, help="sequences per GPU")
     ap.add_argument("--steps", type=int, default=10)
     ap.add_argument("--depth", type=int, default=-1, help="Strassen depth of the Linears (-1 = tuner table)")
+    ap.add_argument("--fused", action="store_true", help="norms, activations, residuals and loss on the library too")
+    ap.add_argument("--clip", type=float, default=0.0, help="clip gradients to this norm (0 = off)")
     args = ap.parse_args()
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))
@@ -167,12 +194,13 @@ def main():
         dist.init_process_group("nccl", rank=rank, world_size=world, device_id=torch.device("cuda", local))
     from . import _lib
 
-    model = build(args.layers, args.seq, None if args.depth < 0 else args.depth, "cuda", world)
-    train_steps(model, 2, args.batch, args.seq, rank)          # warm-up
+    model = build(args.layers, args.seq, None if args.depth < 0 else args.depth, "cuda", world,
+                  fused=args.fused)
+    train_steps(model, 2, args.batch, args.seq, rank, clip=args.clip)          # warm-up
     torch.cuda.synchronize()
     launches = _lib.load().b200s_launch_count()
     t0 = time.perf_counter()
-    losses = train_steps(model, args.steps, args.batch, args.seq, rank)
+    losses = train_steps(model, args.steps, args.batch, args.seq, rank, clip=args.clip)
     torch.cuda.synchronize()
     dt = time.perf_counter() - t0
     if rank == 0:

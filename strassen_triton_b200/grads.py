@@ -1,0 +1,149 @@
+"""The global gradient norm over many tensors and clipping to it: `grad_norm`, `clip_grads_` on a list of
+gradients, `clip_grad_norm_` on parameters (torch.nn.utils' name and formula).
+
+Two launches for a whole model (every 128 tensors), no synchronisation, no copy of the gradients: the
+sum of squares (in fp64), then one pass that forms the coefficient on the device and scales. When the
+norm is below the bound that pass reads and writes nothing.
+"""
+from __future__ import annotations
+
+import math
+from typing import Iterable, Optional, Sequence
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from ._call import DTYPE, call, require_cuda
+
+
+def _dense(t: Tensor) -> bool:
+    """Do the elements of ``t`` fill one gapless span of memory, each once (in any order)?"""
+    if t.is_contiguous():
+        return True
+    need = 1
+    for size, stride in sorted(zip(t.shape, t.stride()), key=lambda x: x[1]):
+        if size == 1:
+            continue
+        if stride != need:
+            return False
+        need *= size
+    return True
+
+
+def _checked(grads: Sequence[Tensor], what: str):
+    if not grads:
+        raise ValueError(f"{what} is empty")
+    dev = grads[0].device if isinstance(grads[0], Tensor) else None
+    for t in grads:
+        if not isinstance(t, Tensor) or not t.is_cuda or t.device != dev:
+            require_cuda(grads[0], t)
+        if t.dtype not in DTYPE:
+            raise TypeError(f"unsupported dtype {t.dtype} in {what} (bfloat16, float16 and float32 are supported)")
+        if t.layout is not torch.strided:
+            raise TypeError(f"{what} must hold dense tensors")
+    return dev
+
+
+def _entries(src, dst):
+    n = len(src)
+    arr = (_lib.TensorEntry * n)()
+    for e, s, d in zip(arr, src, dst):
+        e.src, e.dst, e.numel = s.data_ptr(), d.data_ptr(), s.numel()
+        e.dtype, e.dst_dtype = DTYPE[s.dtype], DTYPE[d.dtype]
+    return arr
+
+
+def _sumsq(dev, arr, n, group):
+    """(parts, how many of them count): the partial sums of squares, of all ranks of ``group`` when given."""
+    parts = torch.empty(_lib.NORM_PARTS, dtype=torch.float64, device=dev)
+    call(dev, _lib.load().b200s_grad_sumsq, arr, n, parts.data_ptr())
+    if group is None:
+        return parts, _lib.NORM_PARTS
+    import torch.distributed as dist
+
+    total = parts.sum().reshape(1)
+    dist.all_reduce(total, group=group)
+    return total, 1
+
+
+def grad_norm(grads: Iterable[Tensor], *, group=None) -> Tensor:
+    """sqrt of the sum of squares over all tensors, a 0-d float32 tensor, on the current stream. ``group``: a
+    process group whose ranks each hold a shard of the gradients; their sums of squares are added."""
+    grads = list(grads)
+    dev = _checked(grads, "grads")
+    flat = [t if _dense(t) else t.contiguous() for t in grads]
+    parts, n_parts = _sumsq(dev, _entries(flat, flat), len(flat), group)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    call(dev, _lib.load().b200s_grad_norm, parts.data_ptr(), n_parts, norm.data_ptr())
+    return norm
+
+
+@torch.no_grad()
+def clip_grads_(grads: Iterable[Tensor], max_norm: float, *, out: Optional[Sequence[Tensor]] = None,
+                error_if_nonfinite: bool = False, group=None) -> Tensor:
+    """Scale ``grads`` in place by min(1, max_norm / (norm + 1e-6)) and return their norm before that (a 0-d
+    float32 tensor, not synchronised).
+
+    ``out``: tensors of the same shapes (any of the supported types, for instance the optimizer's float32
+    gradients) that receive the scaled values instead; the gradients are then only read. A norm that is NaN
+    makes all results NaN, unless ``error_if_nonfinite`` (which waits for the GPU) raises first. ``group`` as in
+    `grad_norm`. A tensor that is written may appear only once and overlap no other one."""
+    grads = list(grads)
+    dev = _checked(grads, "grads")
+    max_norm = float(max_norm)
+    if math.isnan(max_norm) or max_norm < 0:
+        raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
+    src = [t if _dense(t) else t.contiguous() for t in grads]
+    if out is None:
+        for t in grads:
+            if any(st == 0 and sz > 1 for sz, st in zip(t.shape, t.stride())):
+                raise ValueError("a gradient with repeated elements (an expanded tensor) cannot be scaled in place")
+        dst, back = src, [(t, s) for t, s in zip(grads, src) if t is not s]
+    else:
+        out = list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"out holds {len(out)} tensors for {len(grads)} gradients")
+        _checked(out, "out")
+        if out[0].device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {out[0].device}")
+        dst, back = [], []
+        for i, (t, o) in enumerate(zip(grads, out)):
+            if o.shape != t.shape:
+                raise ValueError(f"out[{i}] has shape {tuple(o.shape)}, its gradient {tuple(t.shape)}")
+            if o.is_contiguous():
+                if not src[i].is_contiguous():
+                    src[i] = src[i].contiguous()
+                dst.append(o)
+            elif o.stride() == src[i].stride():
+                dst.append(o)
+            else:
+                src[i] = src[i].contiguous()
+                dst.append(torch.empty(o.shape, dtype=o.dtype, device=dev))
+                back.append((o, dst[-1]))
+    lib = _lib.load()
+    arr = _entries(src, dst)
+    parts, n_parts = _sumsq(dev, arr, len(src), group)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    if error_if_nonfinite:
+        call(dev, lib.b200s_grad_norm, parts.data_ptr(), n_parts, norm.data_ptr())
+        if not math.isfinite(norm.item()):
+            raise RuntimeError("the norm of the gradients is not finite, so they cannot be clipped")
+    call(dev, lib.b200s_grad_clip, arr, len(src), parts.data_ptr(), n_parts, max_norm, norm.data_ptr())
+    for t, s in back:
+        t.copy_(s)
+    return norm
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, *,
+                    group=None) -> Tensor:
+    """torch.nn.utils.clip_grad_norm_ on the library's kernels: clips the ``grad`` of every parameter (those
+    without one are passed over) and returns the norm. Only the 2-norm is offered."""
+    if float(norm_type) != 2.0:
+        raise ValueError(f"only norm_type 2 is offered, got {norm_type}")
+    if isinstance(parameters, Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    return clip_grads_(grads, max_norm, error_if_nonfinite=error_if_nonfinite, group=group)

@@ -6,7 +6,7 @@ The layer stays an ``nn.Linear`` subclass with ordinary parameters, so FSDP
 (``use_orig_params=True``), autocast and ``state_dict`` treat it like any Linear. Differences
 from the reference, all widenings: in_features may differ from out_features, the flattened batch
 may exceed the feature size (no zero padding to D x D is made), and ``depth=None`` / ``-1`` asks the
-tuner table for algorithm and depth.
+tuner table for algorithm and depth; an ``activation`` and a ``residual`` ride in the product's epilogue.
 """
 from __future__ import annotations
 
@@ -21,7 +21,7 @@ from . import ops
 
 class LinearStrassen(nn.Linear):
     def __init__(self, in_features: int, out_features: Optional[int] = None, bias: bool = True, dtype=None,
-                 depth: Optional[int] = 1, device="cuda", algo: str = "classic") -> None:
+                 depth: Optional[int] = 1, device="cuda", algo: str = "classic", activation: str = "none") -> None:
         # main_profiling.py:51-60 spells the constructor (features, bias, dtype, depth, device)
         if isinstance(out_features, bool):
             # every later positional argument sits one slot to the left in that spelling
@@ -32,10 +32,14 @@ class LinearStrassen(nn.Linear):
         if out_features is None:
             out_features = in_features
         super().__init__(in_features, out_features, bias, device, dtype)
+        if activation not in ops.ACTIVATIONS:
+            raise ValueError(f"activation must be one of {sorted(ops.ACTIVATIONS)}, got {activation!r}")
         self.depth = depth
         self.algo = algo
+        self.activation = activation
 
-    def forward(self, input: Tensor) -> Tensor:
+    def forward(self, input: Tensor, residual: Optional[Tensor] = None) -> Tensor:
+        """activation(input @ weight.T + bias) + residual; with no activation and no residual, the plain layer."""
         *batch_dims, d_in = input.shape
         assert d_in == self.in_features, "Input dim mismatch"
         x = input.reshape(-1, d_in)
@@ -57,6 +61,13 @@ class LinearStrassen(nn.Linear):
                 depth -= 1
             if depth == 0:
                 algo = "dense"
+        if self.activation != "none" or residual is not None:
+            if residual is not None and residual.dtype != x.dtype:
+                residual = residual.to(x.dtype)
+            if residual is not None:
+                residual = residual.reshape(-1, self.out_features)
+            out = ops.linear_act(x, w, self.bias, self.activation, residual, algo=algo, depth=depth)
+            return out.view(*batch_dims, self.out_features)
         # weight.T stays a view (model/layers.py:252); the bias rides in the product's epilogue
         # instead of a separate pass over the output (model/layers.py:271-272)
         if self.bias is not None:

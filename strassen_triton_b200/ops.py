@@ -12,7 +12,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _call, _lib
 
 _DTYPE = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
 _ALGO = {"auto": _lib.ALGO_AUTO, "dense": _lib.ALGO_DENSE, "classic": _lib.ALGO_CLASSIC,
@@ -292,3 +292,219 @@ def matmul_autograd(X, W, algo="auto", depth=-1, prod_dtype=None):
     """Differentiable X @ W (2-D or batched 3-D operands); traceable by torch.compile."""
     _require_cuda(X, W)
     return _matmul_op(X, W, algo, int(depth), _DT_NAME[prod_dtype])
+
+
+# ---- linear layer with bias, activation and residual in the product's epilogue --------------------
+ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "relu2": _lib.ACT_RELU2, "silu": _lib.ACT_SILU,
+               "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """A 2-D operand whose rows (or columns) TMA can address: ``t`` itself, or a copy with its rows padded
+    to whole 16-byte vectors. The padding is never read: the product's extents stay those of ``t``."""
+    es = t.element_size()
+    sr, sc = t.stride()
+    if t.data_ptr() % 16 == 0:
+        if sc == 1 and sr >= t.shape[1] and sr * es % 16 == 0:
+            return t
+        if sr == 1 and sc >= t.shape[0] and sc * es % 16 == 0:
+            return t
+    if sr == 1 and sc > 1:
+        return _aligned(t.t()).t()
+    v = 16 // es
+    out = torch.empty((t.shape[0], (t.shape[1] + v - 1) // v * v), dtype=t.dtype, device=t.device)[:, :t.shape[1]]
+    return out.copy_(t)
+
+
+def _split_k(t: torch.Tensor, dim: int) -> torch.Tensor:
+    """fp32 operands run as three TF32 passes over K segments of whole 16-byte vectors: zeros up to those."""
+    if t.dtype != torch.float32 or t.shape[dim] % 4 == 0:
+        return t
+    pad = -t.shape[dim] % 4
+    return torch.nn.functional.pad(t, (0, pad) if dim == 1 else (0, 0, 0, pad))
+
+
+def _epilogue_product(A, B, C, activation, bias, residual, preact, algo, depth, precision):
+    """C = act(A @ B + bias) + residual on 2-D operands, z into ``preact`` when given."""
+    A, B = _aligned(_split_k(A, 1)), _aligned(_split_k(B, 0))
+    p, A, B = make_problem(A, B, C, algo, depth, 0, None, precision)
+    e = _lib.Epilogue()
+    e.activation = activation
+    if bias is not None:
+        e.bias = bias.data_ptr()
+    if residual is not None:
+        e.residual, e.ld_residual = residual.data_ptr(), residual.stride(0)
+    if preact is not None:
+        e.preact, e.ld_preact = preact.data_ptr(), preact.stride(0)
+    lib = _lib.load()
+    n = ctypes.c_size_t(0)
+    pp, pe = ctypes.byref(p), ctypes.byref(e)
+    rc = lib.b200s_matmul_epilogue_workspace(pp, pe, ctypes.byref(n))
+    if rc:
+        _lib.check(rc)
+    ws = torch.empty(n.value, dtype=torch.uint8, device=C.device) if n.value else None
+    _call.call(C.device, lib.b200s_matmul_epilogue, pp, pe, A.data_ptr(), B.data_ptr(), C.data_ptr(),
+               ws.data_ptr() if ws is not None else None, n.value)
+    return C
+
+
+def _linear_act_forward(x, weight, bias, residual, act, algo, depth, precision, save):
+    """(y, z) of 2-D x; z (what the backward pass needs of the pre-activation) is None for "none" or without
+    ``save``."""
+    M, N = x.shape[0], weight.shape[0]
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    z = torch.empty((M, N), dtype=x.dtype, device=x.device) if save and act != _lib.ACT_NONE else None
+    if M:
+        r = residual
+        if r is not None and ((r.stride(1) != 1 and N > 1) or r.stride(0) < 0):
+            r = r.contiguous()
+        _epilogue_product(x, weight.t(), y, act, bias, r, z, algo, depth, precision)
+    return y, z
+
+
+def _linear_act_backward(dy, x, weight, z, act, algo, depth, precision, need_x, need_w, need_b):
+    """(dx, dw, db) of 2-D dy and x, None where not needed."""
+    M, N = dy.shape
+    K = x.shape[1]
+    if dy.dtype != x.dtype:
+        dy = dy.to(x.dtype)
+    if M == 0:
+        return (torch.empty_like(x) if need_x else None, torch.zeros_like(weight) if need_w else None,
+                weight.new_zeros(N) if need_b else None)
+    if (dy.stride(1) != 1 and N > 1) or dy.stride(0) < 0:
+        dy = dy.contiguous()
+    lib, dev = _lib.load(), x.device
+    dz, db = dy, None
+    products = need_x or need_w
+    if act != _lib.ACT_NONE or need_b:
+        out = None
+        if act != _lib.ACT_NONE and products:
+            v = 16 // x.element_size()
+            out = torch.empty((M, (N + v - 1) // v * v), dtype=x.dtype, device=dev)[:, :N]
+            dz = out
+        ws, need = None, 0
+        if need_b:
+            db = torch.empty(N, dtype=x.dtype, device=dev)
+            n = ctypes.c_size_t(0)
+            _lib.check(lib.b200s_epilogue_backward_workspace(M, N, ctypes.byref(n)))
+            need = n.value
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        if out is not None or db is not None:
+            _call.call(dev, lib.b200s_epilogue_backward, M, N, _DTYPE[x.dtype], act, _call.ptr(z),
+                       z.stride(0) if z is not None else 0, dy.data_ptr(), dy.stride(0), _call.ptr(out),
+                       out.stride(0) if out is not None else 0, _call.ptr(db), _call.ptr(ws), need)
+    dx = dw = None
+    if products:
+        dz = _aligned(dz)
+    if need_x:
+        dx = torch.empty((M, K), dtype=x.dtype, device=dev)
+        _epilogue_product(dz, weight, dx, _lib.ACT_NONE, None, None, None, algo, depth, precision)
+    if need_w:
+        dw = torch.empty((N, K), dtype=x.dtype, device=dev)
+        _epilogue_product(dz.t(), x, dw, _lib.ACT_NONE, None, None, None, algo, depth, precision)
+    return dx, dw, db
+
+
+class _LinearActFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, algo, depth, precision):
+        need = ctx.needs_input_grad
+        y, z = _linear_act_forward(x, weight, bias, residual, act, algo, depth, precision, any(need[:3]))
+        ctx.save_for_backward(x, weight, z)
+        ctx.cfg = (act, algo, depth, precision)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if any(need[:3]):
+            dx, dw, db = _linear_act_backward(dy, x, weight, z, *ctx.cfg, *need[:3])
+        return dx, dw, db, dy if need[3] else None, None, None, None, None
+
+
+@torch.library.custom_op("b200s::linear_act", mutates_args=())
+def _linear_act_op(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
+                   residual: Optional[torch.Tensor], act: int, algo: str, depth: int,
+                   precision: str) -> tuple[torch.Tensor, torch.Tensor]:
+    y, z = _linear_act_forward(x, weight, bias, residual, act, algo, depth, precision or None, True)
+    return y, (x.new_empty(0) if z is None else z)
+
+
+@_linear_act_op.register_fake
+def _(x, weight, bias, residual, act, algo, depth, precision):
+    shape = (x.shape[0], weight.shape[0])
+    return x.new_empty(shape), x.new_empty(shape if act != _lib.ACT_NONE else (0,))
+
+
+@torch.library.custom_op("b200s::linear_act_backward", mutates_args=())
+def _linear_act_backward_op(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, z: torch.Tensor, act: int,
+                            algo: str, depth: int, precision: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _linear_act_backward(dy, x, weight, z if act != _lib.ACT_NONE else None, act, algo, depth, precision or None,
+                                True, True, True)
+
+
+@_linear_act_backward_op.register_fake
+def _(dy, x, weight, z, act, algo, depth, precision):
+    return x.new_empty(x.shape), weight.new_empty(weight.shape), weight.new_empty((weight.shape[0],))
+
+
+def _linear_act_setup(ctx, inputs, output):
+    x, weight, bias, residual, act, algo, depth, precision = inputs
+    ctx.save_for_backward(x, weight, output[1])
+    ctx.cfg = (act, algo, depth, precision)
+    ctx.has = (bias is not None, residual is not None)
+
+
+def _linear_act_op_backward(ctx, dy, _dz):
+    x, weight, z = ctx.saved_tensors
+    dx, dw, db = _linear_act_backward_op(dy, x, weight, z, *ctx.cfg)
+    return dx, dw, db if ctx.has[0] else None, dy if ctx.has[1] else None, None, None, None, None
+
+
+_linear_act_op.register_autograd(_linear_act_op_backward, setup_context=_linear_act_setup)
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
+               residual: Optional[torch.Tensor] = None, *, algo: str = "dense", depth: int = 0,
+               precision: Optional[str] = None) -> torch.Tensor:
+    """act(x @ weight.T + bias) + residual as one call, on the current CUDA stream.
+
+    x: (..., K), weight: (N, K), bias: (N,) or None, residual: (..., N) or None; activation one of ``ACTIVATIONS``.
+    All of one type (bias is converted); rows may be strided and of any length (operand rows that are not whole
+    16-byte vectors are copied). Everything after the product is fp32 and rounded once. Differentiable once in all
+    four; for the backward pass the pre-activation is kept in x's type. ``algo``, ``depth`` and ``precision`` choose
+    the products, forward and backward, as in `matmul`."""
+    _call.require_cuda(x, weight, bias, residual)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    if x.dtype not in _DTYPE or weight.dtype != x.dtype:
+        raise TypeError(f"unsupported operand dtypes {x.dtype}, {weight.dtype}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not form x @ weight.T")
+    if algo not in _ALGO:
+        raise ValueError(f"algo must be one of {sorted(_ALGO)}, got {algo!r}")
+    out_shape = x.shape[:-1] + (weight.shape[0],)
+    if bias is not None:
+        if bias.shape != out_shape[-1:]:
+            raise ValueError(f"bias must hold {out_shape[-1]} elements, got shape {tuple(bias.shape)}")
+        bias = bias.to(x.dtype).contiguous()
+    if residual is not None:
+        if residual.shape != out_shape:
+            raise ValueError(f"residual must have the shape of the result {tuple(out_shape)}, got {tuple(residual.shape)}")
+        if residual.dtype != x.dtype:
+            raise TypeError(f"residual must be of the type of x ({x.dtype}), got {residual.dtype}")
+        if residual.dim() != 2:
+            residual = residual.reshape(-1, out_shape[-1])
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    depth = int(depth)
+    if torch.compiler.is_compiling():
+        y = _linear_act_op(x2, weight, bias, residual, act, algo, depth, precision or "")[0]
+    elif _call.wants_grad(x, weight, bias, residual):
+        y = _LinearActFn.apply(x2, weight, bias, residual, act, algo, depth, precision)
+    else:
+        y = _linear_act_forward(x2, weight, bias, residual, act, algo, depth, precision, False)[0]
+    return y if x.dim() == 2 else y.view(out_shape)
