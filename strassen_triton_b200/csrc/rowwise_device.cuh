@@ -46,6 +46,81 @@ struct alignas(sizeof(T) * VEC) Pack {
   T e[VEC];
 };
 
+// ---- pairs of fp32 values ------------------------------------------------------------------------
+// sm_100 adds, multiplies and fuses two fp32 values per instruction (each lane rounded as the scalar
+// form rounds). The single-float overloads let one body serve vectors of one element.
+__device__ __forceinline__ uint64_t f2_bits(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 bits_f2(uint64_t b) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(b));
+  return v;
+}
+__device__ __forceinline__ float2 fma_(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+  return bits_f2(r);
+}
+__device__ __forceinline__ float2 add_(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return bits_f2(r);
+}
+__device__ __forceinline__ float2 mul_(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return bits_f2(r);
+}
+__device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float add_(float a, float b) { return a + b; }
+__device__ __forceinline__ float mul_(float a, float b) { return a * b; }
+__device__ __forceinline__ float hsum(float2 a) { return a.x + a.y; }
+__device__ __forceinline__ float hsum(float a) { return a; }
+
+// The arithmetic unit of vectors of VEC elements: a pair, or one value.
+template <int VEC>
+struct Unit {
+  using type = float2;
+  static constexpr int n = 2, count = VEC / 2;
+  static __device__ __forceinline__ float2 all(float v) { return make_float2(v, v); }
+};
+template <>
+struct Unit<1> {
+  using type = float;
+  static constexpr int n = 1, count = 1;
+  static __device__ __forceinline__ float all(float v) { return v; }
+};
+
+// Two neighbouring elements <-> a pair.
+__device__ __forceinline__ float2 load2(const __nv_bfloat16* e) {
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(e);
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ float2 load2(const __half* e) { return __half22float2(*reinterpret_cast<const __half2*>(e)); }
+__device__ __forceinline__ float2 load2(const float* e) { return *reinterpret_cast<const float2*>(e); }
+__device__ __forceinline__ void store2(__nv_bfloat16* e, float2 v) { *reinterpret_cast<__nv_bfloat162*>(e) = __float22bfloat162_rn(v); }
+__device__ __forceinline__ void store2(__half* e, float2 v) { *reinterpret_cast<__half2*>(e) = __float22half2_rn(v); }
+__device__ __forceinline__ void store2(float* e, float2 v) { *reinterpret_cast<float2*>(e) = v; }
+
+// Unit k of a vector.
+template <typename T, int VEC>
+__device__ __forceinline__ typename Unit<VEC>::type unit_of(const Pack<T, VEC>& v, int k) {
+  if constexpr (VEC == 1)
+    return to_f(v.e[0]);
+  else
+    return load2(v.e + 2 * k);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void set_unit(Pack<T, VEC>& v, int k, typename Unit<VEC>::type u) {
+  if constexpr (VEC == 1)
+    v.e[0] = from_f<T>(u);
+  else
+    store2(v.e + 2 * k, u);
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
