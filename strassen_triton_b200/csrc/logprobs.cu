@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include "common.h"
+#include "ptx_sm100.cuh"
 #include "rowwise_device.cuh"
 
 namespace b200s {
@@ -82,6 +83,31 @@ __device__ __forceinline__ uint64_t cand_word(uint32_t key, uint32_t idx) {
   return (static_cast<uint64_t>(key) << 32) | (0xffffffffu - idx);
 }
 
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+}
+// Values at the same shared-memory place in CTA `cta` of the cluster.
+__device__ __forceinline__ uint64_t ld_cluster_u64(const void* place, int cta) {
+  uint64_t v;
+  asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(ptx::mapa_cluster(ptx::smem_u32(place), cta)) : "memory");
+  return v;
+}
+__device__ __forceinline__ Stats ld_cluster_stats(const Stats* place, int cta) {
+  const uint32_t at = ptx::mapa_cluster(ptx::smem_u32(place), cta);
+  Stats a;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a.m) : "r"(at) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a.s) : "r"(at + 4) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a.u) : "r"(at + 8) : "memory");
+  return a;
+}
+
 struct LogprobFwd {
   const void* logits;
   const int64_t* targets;
@@ -92,65 +118,336 @@ struct LogprobFwd {
   float* top_logprobs;
   int64_t rows, ld, ignore_index;
   int32_t vocab, top_k;
+  int32_t parts;       // CTAs (a cluster) that share a row
 };
 
+// The elements of a row as a head up to the first 16-byte boundary, a body of 16-byte vectors and a tail.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprob_fwd_kernel(const LogprobFwd p) {
+struct RowSpan {
+  static constexpr int V = 16 / sizeof(T);
+  int head, vecs, n;
+  __device__ __forceinline__ RowSpan(const T* x, int n_) : n(n_) {
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+    head = off == 0 ? 0 : V - off;
+    if (head > n) head = n;
+    vecs = (n - head) / V;
+  }
+  __device__ __forceinline__ int tail() const { return head + vecs * V; }
+};
+
+using row::Pack;
+
+// Adds a batch of B vectors to the running statistics: one look for a larger maximum per batch.
+template <typename T, bool ENT, int B>
+__device__ __forceinline__ void add_batch(Stats& a, const Pack<T, 16 / sizeof(T)> (&v)[B], float2& s2, float2& u2) {
+  constexpr int V = 16 / sizeof(T);
+  float top = kNegInf;
+#pragma unroll
+  for (int b = 0; b < B; ++b)
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      const float2 x = row::load2(v[b].e + 2 * k);
+      top = fmaxf(top, fmaxf(x.x, x.y));
+    }
+  if (top > a.m) {
+    // move what is summed so far to the new maximum
+    a.s = s2.x + s2.y;
+    a.u = ENT ? u2.x + u2.y : 0.f;
+    rescale(a, top);
+    s2 = make_float2(a.s, 0.f);
+    u2 = make_float2(a.u, 0.f);
+  }
+  const float shift = a.m == kNegInf ? 0.f : -a.m;      // nothing finite yet: only -inf (adds 0) or NaN
+  const float2 sh = make_float2(shift, shift), l2 = make_float2(kLog2e, kLog2e);
+#pragma unroll
+  for (int b = 0; b < B; ++b)
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      const float2 d = row::add_(row::load2(v[b].e + 2 * k), sh);
+      const float2 t = row::mul_(d, l2);
+      const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+      s2 = row::add_(s2, e);
+      // e is 0 long before -1000: a forbidden token adds 0, not 0 * inf
+      if constexpr (ENT) u2 = row::fma_(e, make_float2(fmaxf(d.x, -1000.f), fmaxf(d.y, -1000.f)), u2);
+    }
+}
+
+constexpr int kCandidates = 2048;
+
+// Scratch of the selection of the best alternatives.
+struct TopShared {
+  uint64_t cand[kCandidates];
+  uint64_t best[kMaxTopK];         // of this CTA
+  int count;
+  int warp_count[kThreads / 32];
+};
+
+// f(index, value) for the elements of vectors v0 .. v1 of a row, plus head and tail of a first and a last part, that
+// are not below `least` (a NaN is not).
+template <typename T, typename F>
+__device__ __forceinline__ void for_elements(const T* x, const RowSpan<T>& sp, int v0, int v1, bool first_part, bool last_part,
+                                             float least, F&& f) {
+  constexpr int V = RowSpan<T>::V, B = 4;
+  auto one = [&](int c) {
+    const float v = to_f(x[c]);
+    if (!(v < least)) f(c, v);
+  };
+  if (first_part && static_cast<int>(threadIdx.x) < sp.head) one(threadIdx.x);
+  if (last_part && sp.tail() + static_cast<int>(threadIdx.x) < sp.n) one(sp.tail() + threadIdx.x);
+  auto look = [&](int i, const uint4& q) {
+    const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(&q);
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < V; ++e) any |= !(to_f(v.e[e]) < least);
+    if (any) {        // rare: from memory again, in little code
+      const int c = sp.head + i * V;
+#pragma unroll 1
+      for (int e = 0; e < V; ++e) one(c + e);
+    }
+  };
+  const uint4* body = reinterpret_cast<const uint4*>(x + sp.head);
+  int i = v0 + threadIdx.x;
+  for (; i + (B - 1) * kThreads < v1; i += B * kThreads) {
+    uint4 q[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) q[b] = __ldg(body + i + b * kThreads);
+#pragma unroll
+    for (int b = 0; b < B; ++b) look(i + b * kThreads, q[b]);
+  }
+  uint4 q[B];
+#pragma unroll
+  for (int b = 0; b < B; ++b)
+    if (i + b * kThreads < v1) q[b] = __ldg(body + i + b * kThreads);
+#pragma unroll
+  for (int b = 0; b < B; ++b)
+    if (i + b * kThreads < v1) look(i + b * kThreads, q[b]);
+}
+
+// The k best of this CTA's part, best first, into out[0 .. k); fewer elements leave zeros. `mine` is the
+// largest value this thread saw. The k-th largest of the threads' maxima bounds the k-th best from below (its
+// upper 16 bits do, found bit by bit), so one more pass collects the few elements at or above that bound and
+// ranks them. When too many share that bound
+// (a masked row, few distinct values) only those above it are collected, and the lowest ids of those equal to it
+// are found in order; when even those above it are too many, the k best are searched one after the other.
+template <typename T>
+__device__ __noinline__ void select_best(const T* x, const RowSpan<T>& sp, int v0, int v1, bool first_part, bool last_part, float mine, int k,
+                            TopShared& sh, uint64_t* out) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) sh.count = 0;
+  for (int i = tid; i < k; i += kThreads) out[i] = 0;
+  const uint32_t own = order_key(mine);
+  uint32_t bound = 0;
+#pragma unroll 1
+  for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
+    if (__syncthreads_count(own >= (bound | bit)) >= k) bound |= bit;
+  const uint32_t forbidden = order_key(kNegInf);
+  auto collect = [&](uint32_t at_least) {
+    for_elements<T>(x, sp, v0, v1, first_part, last_part, key_value(at_least), [&](int c, float v) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCandidates) sh.cand[at] = cand_word(order_key(v), c);
+    });
+  };
+  int n = kCandidates + 1;
+  if (bound > forbidden) {
+    collect(bound);
+    __syncthreads();
+    n = sh.count;
+    __syncthreads();
+  }
+  if (n > kCandidates) {
+    if (bound <= forbidden) {
+      bound = forbidden;      // fewer than k threads saw an allowed token: those, then forbidden ones
+    } else {
+      // the exact k-th largest maximum
+#pragma unroll 1
+      for (uint32_t bit = 1u << 15; bit != 0; bit >>= 1)
+        if (__syncthreads_count(own >= (bound | bit)) >= k) bound |= bit;
+    }
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    if (bound != 0xffffffffu) collect(bound + 1);     // above a NaN there is nothing
+    __syncthreads();
+    n = sh.count;
+    __syncthreads();
+    if (n <= kCandidates) {
+      // the lowest ids whose key equals the bound, in order, until there are k candidates
+      int have = n;
+      const int c0 = first_part ? 0 : sp.head + v0 * RowSpan<T>::V, c1 = last_part ? sp.n : sp.head + v1 * RowSpan<T>::V;
+      for (int base = c0; base < c1 && have < k; base += kThreads) {
+        const int c = base + tid;
+        const bool hit = c < c1 && order_key(to_f(x[c])) == bound;
+        const uint32_t mask = __ballot_sync(0xffffffffu, hit);
+        if (lane == 0) sh.warp_count[warp] = __popc(mask);
+        __syncthreads();
+        int before = __popc(mask & ((1u << lane) - 1)), total = 0;
+        for (int w = 0; w < kThreads / 32; ++w) {
+          const int cnt = sh.warp_count[w];
+          if (w < warp) before += cnt;
+          total += cnt;
+        }
+        if (hit && have + before < kCandidates) sh.cand[have + before] = cand_word(bound, c);
+        have += total;
+        __syncthreads();
+      }
+      n = have < kCandidates ? have : kCandidates;
+    } else {
+      uint64_t last = ~uint64_t{0};
+      for (int i = 0; i < k; ++i) {
+        uint64_t top = 0;
+        for_elements<T>(x, sp, v0, v1, first_part, last_part, kNegInf, [&](int c, float v) {
+          const uint64_t w = cand_word(order_key(v), c);
+          if (w < last && w > top) top = w;
+        });
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const uint64_t other = __shfl_xor_sync(0xffffffffu, top, o);
+          if (other > top) top = other;
+        }
+        if (lane == 0) sh.cand[warp] = top;
+        __syncthreads();
+        for (int w = 0; w < kThreads / 32; ++w)
+          if (sh.cand[w] > top) top = sh.cand[w];
+        last = top;
+        if (tid == 0) out[i] = top;
+        __syncthreads();
+      }
+      return;
+    }
+  }
+  // words are distinct: a candidate's rank is the number of larger ones
+  for (int i = tid; i < n; i += kThreads) {
+    const uint64_t w = sh.cand[i];
+    int rank = 0;
+    for (int j = 0; j < n && rank < k; ++j) rank += sh.cand[j] > w;
+    if (rank < k) out[rank] = w;
+  }
+  __syncthreads();
+}
+
+// (Five resident blocks keep enough loads on their way; the selection stays out of line, or its registers would
+// leave room for one.)
+template <typename T, bool ENT, bool TOP>
+__global__ void __launch_bounds__(kThreads, 5) logprob_fwd_kernel(const LogprobFwd p) {
+  constexpr int V = 16 / sizeof(T);
+  constexpr int B = 32 / V;            // 32 elements a thread on their way
   __shared__ Stats warp_stats[kThreads / 32];
-  __shared__ uint64_t best[kThreads / 32];
+  __shared__ Stats part_stats;
+  __shared__ float2 row_result;        // maximum and log of the sum
+  extern __shared__ __align__(16) uint8_t top_raw[];
+  TopShared& top = *reinterpret_cast<TopShared*>(top_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+  const int parts = p.parts;
+  const int part = parts > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
+  const bool first_part = part == 0, last_part = part == parts - 1;
+  for (int64_t r = blockIdx.x / parts; r < p.rows; r += gridDim.x / parts) {
     const T* x = static_cast<const T*>(p.logits) + r * p.ld;
+    const RowSpan<T> sp(x, p.vocab);
+    const int per = (sp.vecs + parts - 1) / parts;
+    const int v0 = min(part * per, sp.vecs), v1 = min(v0 + per, sp.vecs);
     Stats a = empty_stats();
-    for (int c = threadIdx.x; c < p.vocab; c += kThreads) {
+    float2 s2 = make_float2(0.f, 0.f), u2 = s2;
+    const Pack<T, V>* body = reinterpret_cast<const Pack<T, V>*>(x + sp.head);
+    int i = v0 + threadIdx.x;
+    for (; i + (B - 1) * kThreads < v1; i += B * kThreads) {
+      Pack<T, V> v[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b) v[b] = body[i + b * kThreads];
+      add_batch<T, ENT, B>(a, v, s2, u2);
+    }
+    if (v1 - v0 >= 4 * B * kThreads) {
+      // what is left of a long part: a few vectors, one by one
+      for (; i < v1; i += kThreads) {
+        const Pack<T, V> v[1] = {body[i]};
+        add_batch<T, ENT, 1>(a, v, s2, u2);
+      }
+    } else if (i < v1) {
+      // of a short one, where each wait counts: one more batch, filled up with forbidden tokens
+      Pack<T, V> v[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        if (i + b * kThreads < v1) {
+          v[b] = body[i + b * kThreads];
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[b].e[e] = from_f<T>(kNegInf);
+        }
+      }
+      add_batch<T, ENT, B>(a, v, s2, u2);
+    }
+    a.s = s2.x + s2.y;
+    a.u = ENT ? u2.x + u2.y : 0.f;
+    auto add_one = [&](int c) {
       const float v = to_f(x[c]);
       if (v > a.m) rescale(a, v);
       add(a, v);
-    }
+    };
+    if (first_part && static_cast<int>(threadIdx.x) < sp.head) add_one(threadIdx.x);
+    if (last_part && sp.tail() + static_cast<int>(threadIdx.x) < sp.n) add_one(sp.tail() + threadIdx.x);
+    const float mine = a.m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a = merge(a, shfl_xor(a, o));
     if (lane == 0) warp_stats[warp] = a;
     __syncthreads();
-    a = warp_stats[0];
-    for (int w = 1; w < kThreads / 32; ++w) a = merge(a, warp_stats[w]);
-    const float lse = a.m == kNegInf && a.s == 0.f ? kNegInf : (a.m == kNegInf ? nan_f() : a.m + logf(a.s));
-    if (threadIdx.x == 0) {
-      const int64_t t = p.targets[r];
-      float lp = nan_f();
-      if (t == p.ignore_index) {
-        lp = 0.f;
-      } else if (t >= 0 && t < p.vocab) {
-        const float xt = to_f(x[t]);
-        lp = lse == kNegInf ? kNegInf : (xt - a.m) - logf(a.s);
-      }
-      p.logprob[r] = lp;
-      if (p.lse) p.lse[r] = lse;
-      if (p.entropy) p.entropy[r] = lse == kNegInf ? 0.f : logf(a.s) - a.u / a.s;
-    }
-    // the k best, one after the other: the largest word below the last one found
-    uint64_t last = ~uint64_t{0};
-    for (int k = 0; k < p.top_k; ++k) {
-      uint64_t mine = 0;
-      for (int c = threadIdx.x; c < p.vocab; c += kThreads) {
-        const uint64_t w = cand_word(order_key(to_f(x[c])), c);
-        if (w < last && w > mine) mine = w;
-      }
+    if (warp == 0) {
+      a = lane < kThreads / 32 ? warp_stats[lane] : empty_stats();
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t other = __shfl_xor_sync(0xffffffffu, mine, o);
-        if (other > mine) mine = other;
+      for (int o = kThreads / 64; o > 0; o >>= 1) a = merge(a, shfl_xor(a, o));
+    }
+    if constexpr (TOP) select_best<T>(x, sp, v0, v1, first_part, last_part, mine, p.top_k, top, top.best);
+    if (parts > 1) {
+      // the first CTA of the cluster gathers statistics and candidates of the others from their shared memory
+      if (threadIdx.x == 0) part_stats = a;
+      cluster_sync();
+      if (first_part && warp == 0) {
+        a = lane < parts ? ld_cluster_stats(&part_stats, lane) : empty_stats();
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) a = merge(a, shfl_xor(a, o));
       }
-      if (lane == 0) best[warp] = mine;
-      __syncthreads();
-      for (int w = 0; w < kThreads / 32; ++w)
-        if (best[w] > mine) mine = best[w];
-      last = mine;
+      if constexpr (TOP) {
+        if (first_part)
+          for (int j = threadIdx.x; j < parts * p.top_k; j += kThreads) {
+            const int from = j / p.top_k, at = j - from * p.top_k;
+            top.cand[j] = ld_cluster_u64(&top.best[at], from);
+          }
+      }
+      cluster_sync();      // the others may go on (or leave) once everything has been read
+    }
+    if (first_part) {
       if (threadIdx.x == 0) {
-        const float v = key_value(static_cast<uint32_t>(mine >> 32));
-        p.top_ids[r * p.top_k + k] = 0xffffffffu - static_cast<uint32_t>(mine);
-        p.top_logprobs[r * p.top_k + k] = lse == kNegInf ? kNegInf : (v - a.m) - logf(a.s);
+        const float logs = logf(a.s);
+        const float lse = a.m == kNegInf ? (a.s == 0.f ? kNegInf : nan_f()) : a.m + logs;
+        const int64_t t = p.targets[r];
+        float lp = nan_f();
+        if (t == p.ignore_index) {
+          lp = 0.f;
+        } else if (t >= 0 && t < p.vocab) {
+          lp = lse == kNegInf ? kNegInf : (to_f(x[t]) - a.m) - logs;
+        }
+        p.logprob[r] = lp;
+        if (p.lse) p.lse[r] = lse;
+        if (ENT) p.entropy[r] = lse == kNegInf ? 0.f : logs - a.u / a.s;
+        row_result = make_float2(lse == kNegInf ? kNegInf : a.m, logs);
       }
-      __syncthreads();
+      if constexpr (TOP) {
+        __syncthreads();
+        const float m = row_result.x, logs = row_result.y;
+        auto put = [&](int at, uint64_t w) {
+          p.top_ids[r * p.top_k + at] = 0xffffffffu - static_cast<uint32_t>(w);
+          p.top_logprobs[r * p.top_k + at] = m == kNegInf ? kNegInf : (key_value(static_cast<uint32_t>(w >> 32)) - m) - logs;
+        };
+        if (parts == 1) {
+          for (int j = threadIdx.x; j < p.top_k; j += kThreads) put(j, top.best[j]);
+        } else {
+          const int n = parts * p.top_k;
+          for (int j = threadIdx.x; j < n; j += kThreads) {
+            const uint64_t w = top.cand[j];
+            if (w == 0) continue;       // a part with fewer than top_k elements
+            int rank = 0;
+            for (int q = 0; q < n; ++q) rank += top.cand[q] > w;
+            if (rank < p.top_k) put(rank, w);
+          }
+        }
+      }
     }
     __syncthreads();
   }
@@ -168,28 +465,81 @@ struct LogprobBwd {
   int32_t vocab, width;
 };
 
-template <typename T>
+// One row per block of the grid's first dimension (the last rows first: the forward pass left their logits in
+// L2), its vectors dealt to the blocks of the second.
+template <typename T, bool ENT>
 __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobBwd p) {
-  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    const T* x = static_cast<const T*>(p.logits) + r * p.ld;
-    T* d = static_cast<T*>(p.dlogits) + r * p.ldd;
-    const int64_t t = p.targets[r];
-    const float lse = p.lse[r];
-    const bool ignored = t == p.ignore_index;
-    float gl = p.dlogprob && !ignored ? p.dlogprob[r] : 0.f;
-    const float ge = p.dentropy ? p.dentropy[r] : 0.f;
-    const float h = p.dentropy ? p.entropy[r] : 0.f;
-    if (!ignored && (t < 0 || t >= p.vocab)) gl = nan_f();
-    // an ignored row stays zero whatever its logits hold
-    const bool none = lse == kNegInf || (gl == 0.f && ge == 0.f && (ignored || lse == lse));
-    for (int c = threadIdx.x; c < p.width; c += kThreads) {
-      float v = 0.f;
-      if (!none && c < p.vocab) {
-        const float lp = to_f(x[c]) - lse;
-        const float pr = exp2f(lp * kLog2e);
-        v = gl * ((c == t ? 1.f : 0.f) - pr) - ge * pr * (fmaxf(lp, -1000.f) + h);
+  constexpr int V = 16 / sizeof(T);
+  using P = Pack<T, V>;
+  const int64_t r = p.rows - 1 - blockIdx.x;
+  const T* x = static_cast<const T*>(p.logits) + r * p.ld;
+  T* d = static_cast<T*>(p.dlogits) + r * p.ldd;
+  const int64_t t = p.targets[r];
+  const float lse = p.lse[r];
+  const bool ignored = t == p.ignore_index;
+  float gl = p.dlogprob && !ignored ? p.dlogprob[r] : 0.f;
+  const float ge = ENT ? p.dentropy[r] : 0.f;
+  const float h = ENT ? p.entropy[r] : 0.f;
+  if (!ignored && (t < 0 || t >= p.vocab)) gl = nan_f();
+  const int target = t >= 0 && t < p.vocab && !ignored ? static_cast<int>(t) : -1;
+  // an ignored row stays zero whatever its logits hold
+  const bool none = lse == kNegInf || (gl == 0.f && ge == 0.f && (ignored || lse == lse));
+  const int limit = none ? 0 : p.vocab;
+  auto one = [&](int c) {
+    float v = 0.f;
+    if (c < limit) {
+      const float lp = to_f(x[c]) - lse;
+      const float pr = exp2_approx(lp * kLog2e);
+      v = -gl * pr;
+      if constexpr (ENT) v -= ge * pr * (fmaxf(lp, -1000.f) + h);
+      if (c == target) v += gl;
+    }
+    d[c] = from_f<T>(v);
+  };
+  const int first = static_cast<int>(blockIdx.y) * kThreads + static_cast<int>(threadIdx.x);
+  const int step = static_cast<int>(gridDim.y) * kThreads;
+  const bool paired = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15u) == 0;
+  if (!paired) {
+    for (int c = first; c < p.width; c += step) one(c);
+    return;
+  }
+  const RowSpan<T> sp(d, p.width);
+  if (first < sp.head) one(first);
+  if (sp.tail() + first < p.width) one(sp.tail() + first);
+  const float2 sh = make_float2(-lse, -lse), l2 = make_float2(kLog2e, kLog2e), ng = make_float2(-gl, -gl);
+  const float2 ne = make_float2(-ge, -ge), hh = make_float2(h, h);
+#pragma unroll 4
+  for (int i = first; i < sp.vecs; i += step) {
+    const int c = sp.head + i * V;
+    P out;
+    if (c + V <= limit) {
+      const P v = *reinterpret_cast<const P*>(x + c);
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) {
+        const float2 lp = row::add_(row::load2(v.e + 2 * k), sh);
+        const float2 q = row::mul_(lp, l2);
+        const float2 pr = make_float2(exp2_approx(q.x), exp2_approx(q.y));
+        float2 g = ng;
+        if constexpr (ENT) g = row::fma_(ne, row::add_(make_float2(fmaxf(lp.x, -1000.f), fmaxf(lp.y, -1000.f)), hh), g);
+        row::store2(out.e + 2 * k, row::mul_(g, pr));
       }
-      d[c] = from_f<T>(v);
+      if (static_cast<unsigned>(target - c) < static_cast<unsigned>(V)) {
+        // the target's own column, from fp32 again
+        const float lp = to_f(x[target]) - lse;
+        const float pr = exp2_approx(lp * kLog2e);
+        float w = fmaf(-gl, pr, gl);
+        if constexpr (ENT) w -= ge * pr * (fmaxf(lp, -1000.f) + h);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (c + e == target) out.e[e] = from_f<T>(w);
+      }
+      *reinterpret_cast<P*>(d + c) = out;
+    } else if (c >= limit) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) out.e[e] = from_f<T>(0.f);
+      *reinterpret_cast<P*>(d + c) = out;
+    } else {
+      for (int e = 0; e < V; ++e) one(c + e);
     }
   }
 }
@@ -202,7 +552,65 @@ int check_logits(int64_t rows, int64_t vocab, int dtype) {
 
 bool misaligned(const void* p, size_t es) { return reinterpret_cast<uintptr_t>(p) % es != 0; }
 
-int64_t row_grid(int64_t rows) { return rows < 148 * 64 ? rows : 148 * 64; }
+// CTAs that share a row: as many (a power of two up to 8) as it takes to give every SM two, as long as each
+// keeps 2048 tokens.
+int row_parts(int64_t rows, int64_t vocab) {
+  int n = 1;
+  while (n < 8 && rows * n < 2 * 148 && vocab >= 2 * 2048 * static_cast<int64_t>(n)) n *= 2;
+  return n;
+}
+
+template <typename T, bool ENT, bool TOP>
+int launch_fwd_form(const LogprobFwd& p, cudaStream_t stream) {
+  auto kernel = logprob_fwd_kernel<T, ENT, TOP>;
+  const int64_t cap = 148 * 64;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.rows < cap ? p.rows : cap) * p.parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = TOP ? sizeof(TopShared) : 0;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = static_cast<unsigned>(p.parts);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  B200S_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, p));
+  count_launch();
+  return B200S_OK;
+}
+
+template <typename T>
+int launch_fwd(const LogprobFwd& p, cudaStream_t stream) {
+  if (p.top_k > 0) return p.entropy ? launch_fwd_form<T, true, true>(p, stream) : launch_fwd_form<T, false, true>(p, stream);
+  return p.entropy ? launch_fwd_form<T, true, false>(p, stream) : launch_fwd_form<T, false, false>(p, stream);
+}
+
+template <typename T>
+int launch_bwd(const LogprobBwd& p, cudaStream_t stream) {
+  // a block per row, more when rows are few: at least 2048 columns each
+  int64_t parts = 1;
+  while (p.rows * parts < 4 * 148 && p.width >= 2 * 2048 * parts) parts *= 2;
+  for (int64_t r0 = 0; r0 < p.rows; r0 += int64_t{1} << 30) {
+    LogprobBwd q = p;
+    const int64_t n = p.rows - r0 < (int64_t{1} << 30) ? p.rows - r0 : int64_t{1} << 30;
+    q.rows = n;
+    q.logits = static_cast<const T*>(p.logits) + r0 * p.ld;
+    q.dlogits = static_cast<T*>(p.dlogits) + r0 * p.ldd;
+    q.targets = p.targets + r0, q.lse = p.lse + r0;
+    if (p.entropy) q.entropy = p.entropy + r0;
+    if (p.dlogprob) q.dlogprob = p.dlogprob + r0;
+    if (p.dentropy) q.dentropy = p.dentropy + r0;
+    const dim3 grid(static_cast<unsigned>(n), static_cast<unsigned>(parts));
+    if (p.dentropy)
+      logprob_bwd_kernel<T, true><<<grid, kThreads, 0, stream>>>(q);
+    else
+      logprob_bwd_kernel<T, false><<<grid, kThreads, 0, stream>>>(q);
+    B200S_CUDA_OK(cudaGetLastError());
+    count_launch();
+  }
+  return B200S_OK;
+}
 
 }  // namespace
 
@@ -227,18 +635,11 @@ int b200s_token_logprobs(int64_t rows, int64_t vocab, int dtype, const void* log
     return B200S_ERR_BAD_ALIGNMENT;
   if (!device_status_words()) return B200S_ERR_NO_DEVICE;
   const LogprobFwd p{logits, targets, logprob, lse, entropy, top_ids, top_logprobs, rows, ld, ignore_index,
-                     static_cast<int32_t>(vocab), top_k};
-  const unsigned grid = static_cast<unsigned>(row_grid(rows));
+                     static_cast<int32_t>(vocab), top_k, row_parts(rows, vocab)};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == B200S_BF16)
-    logprob_fwd_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(p);
-  else if (dtype == B200S_FP16)
-    logprob_fwd_kernel<__half><<<grid, kThreads, 0, s>>>(p);
-  else
-    logprob_fwd_kernel<float><<<grid, kThreads, 0, s>>>(p);
-  B200S_CUDA_OK(cudaGetLastError());
-  count_launch();
-  return B200S_OK;
+  if (dtype == B200S_BF16) return launch_fwd<__nv_bfloat16>(p, s);
+  if (dtype == B200S_FP16) return launch_fwd<__half>(p, s);
+  return launch_fwd<float>(p, s);
 }
 
 int b200s_token_logprobs_backward(int64_t rows, int64_t vocab, int64_t width, int dtype, const void* logits, int64_t ld,
@@ -257,17 +658,10 @@ int b200s_token_logprobs_backward(int64_t rows, int64_t vocab, int64_t width, in
   if (!device_status_words()) return B200S_ERR_NO_DEVICE;
   const LogprobBwd p{logits, targets, lse, entropy, dlogprob, dentropy, dlogits, rows, ld, ldd, ignore_index,
                      static_cast<int32_t>(vocab), static_cast<int32_t>(width)};
-  const unsigned grid = static_cast<unsigned>(row_grid(rows));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == B200S_BF16)
-    logprob_bwd_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(p);
-  else if (dtype == B200S_FP16)
-    logprob_bwd_kernel<__half><<<grid, kThreads, 0, s>>>(p);
-  else
-    logprob_bwd_kernel<float><<<grid, kThreads, 0, s>>>(p);
-  B200S_CUDA_OK(cudaGetLastError());
-  count_launch();
-  return B200S_OK;
+  if (dtype == B200S_BF16) return launch_bwd<__nv_bfloat16>(p, s);
+  if (dtype == B200S_FP16) return launch_bwd<__half>(p, s);
+  return launch_bwd<float>(p, s);
 }
 
 }  // extern "C"
