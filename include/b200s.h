@@ -449,7 +449,7 @@ typedef struct b200s_tensor {
   int32_t dst_dtype;  /* b200s_dtype of dst */
 } b200s_tensor;
 
-#define B200S_NORM_PARTS 592
+#define B200S_NORM_PARTS 1184
 
 /*
  * Global gradient norm and clipping. `list` is a host array of `count` tensors (copied into the launches,

@@ -36,7 +36,7 @@ ERR_TOO_LARGE = -13
 ERR_OVERLAP = -14
 
 ACT_NONE, ACT_RELU, ACT_RELU2, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3, 4, 5
-NORM_PARTS = 592
+NORM_PARTS = 1184
 MAX_TOP_K = 64
 
 

@@ -5,13 +5,18 @@
 //
 // A list is cut into chunks of kChunk elements; chunk j of a launch belongs to block j mod grid, so
 // what a block adds up, and in which order, depends on the list alone: results repeat bit for bit.
-// Squares are added in fp64: in fp32 a gradient above 1.8e19 would overflow its square and one below
-// 1e-23 lose it. The list travels in the kernel's parameters, so a captured graph keeps its own copy.
+// The squares of one 16-byte vector are added in fp32 (three roundings at most), everything beyond in
+// fp64; a vector whose sum leaves the safe range of fp32 (a gradient above 2^60 or all below 2^-42) is
+// squared in fp64. The list travels in the kernel's parameters, so a captured graph keeps its own copy.
+//
+// Both passes are bound by memory. The clipping pass takes the chunks last to first: the end of the list
+// is what the norm's pass left in L2 (a model of 326 MB in bf16: about a third of it).
 
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <cstdlib>
+#include <type_traits>
 
 #include "common.h"
 #include "rowwise_device.cuh"
@@ -23,20 +28,24 @@ namespace {
 using row::from_f;
 using row::to_f;
 
-constexpr int kThreads = 256;
-constexpr int kCapacity = 128;     // tensors per launch (the list is a kernel parameter)
-constexpr int kChunk = 16384;      // elements
+using row::Pack;
 
+constexpr int kThreads = 256;
+constexpr int kSmall = 128, kLarge = 512;   // tensors per launch (the list is a kernel parameter, 4 KB or 15 KB)
+constexpr int kChunk = 16384;               // elements
+
+template <int CAP>
 struct ListParams {
-  const void* src[kCapacity];
-  void* dst[kCapacity];
-  int64_t numel[kCapacity];
-  int32_t chunk0[kCapacity + 1];   // first chunk of each tensor
-  uint8_t dtype[kCapacity], dst_dtype[kCapacity];
+  const void* src[CAP];
+  void* dst[CAP];
+  int64_t numel[CAP];
+  int32_t chunk0[CAP + 1];   // first chunk of each tensor
+  uint8_t dtype[CAP], dst_dtype[CAP];
   int32_t count;
 };
 
-__device__ __forceinline__ int find_tensor(const ListParams& p, int chunk) {
+template <int CAP>
+__device__ __forceinline__ int find_tensor(const ListParams<CAP>& p, int chunk) {
   int lo = 0, hi = p.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -59,18 +68,66 @@ __device__ __forceinline__ double block_sum_f64(double v, double* slots) {
   return t;
 }
 
+// Elements from x on up to the first 16-byte boundary.
 template <typename T>
-__device__ __forceinline__ double sumsq_span(const T* x, int64_t n) {
+__device__ __forceinline__ int head_of(const T* x, int n) {
+  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+  const int head = off == 0 ? 0 : static_cast<int>(16 / sizeof(T)) - off;
+  return head < n ? head : n;
+}
+
+template <typename T>
+__device__ __forceinline__ double square(T x) {
+  const double v = static_cast<double>(to_f(x));
+  return v * v;
+}
+
+template <typename T>
+__device__ __forceinline__ double vector_sumsq(const uint4& q) {
+  constexpr int V = 16 / sizeof(T);
+  const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(&q);
+  float2 s[V / 2];
+#pragma unroll
+  for (int k = 0; k < V / 2; ++k) {
+    const float2 t = row::load2(v.e + 2 * k);
+    s[k] = row::mul_(t, t);
+  }
+#pragma unroll
+  for (int w = V / 4; w > 0; w >>= 1)
+#pragma unroll
+    for (int k = 0; k < w; ++k) s[k] = row::add_(s[k], s[k + w]);
+  const float sum = s[0].x + s[0].y;
+  if (sum > 0x1p-84f && sum < 0x1p124f) return static_cast<double>(sum);
+  if (((q.x | q.y | q.z | q.w) & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu)) == 0) return 0.;
+  double d = 0.;
+#pragma unroll
+  for (int e = 0; e < V; ++e) d += square(v.e[e]);
+  return d;
+}
+
+template <typename T>
+__device__ __forceinline__ double sumsq_span(const T* x, int n) {
+  constexpr int V = 16 / sizeof(T), B = 8;
+  const int head = head_of(x, n);
+  const int vecs = (n - head) / V;
+  const int tail = head + vecs * V;
   double a = 0.;
-  for (int64_t i = threadIdx.x; i < n; i += kThreads) {
-    const double v = static_cast<double>(to_f(x[i]));
-    a = fma(v, v, a);
+  if (static_cast<int>(threadIdx.x) < head) a += square(x[threadIdx.x]);
+  if (tail + static_cast<int>(threadIdx.x) < n) a += square(x[tail + threadIdx.x]);
+  const uint4* body = reinterpret_cast<const uint4*>(x + head);
+  for (int i = threadIdx.x; i < vecs; i += B * kThreads) {
+    uint4 q[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) q[b] = i + b * kThreads < vecs ? __ldg(body + i + b * kThreads) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int b = 0; b < B; ++b) a += vector_sumsq<T>(q[b]);
   }
   return a;
 }
 
 // parts[b] (+)= the squares of block b's chunks; the parts of blocks that do not exist are cleared.
-__global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ ListParams p, double* parts, int accumulate) {
+template <int CAP>
+__global__ void __launch_bounds__(kThreads, 5) sumsq_kernel(const __grid_constant__ ListParams<CAP> p, double* parts, int accumulate) {
   __shared__ double slots[kThreads / 32];
   const int chunks = p.chunk0[p.count];
   double a = 0.;
@@ -78,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__
     const int t = find_tensor(p, j);
     const int64_t at = static_cast<int64_t>(j - p.chunk0[t]) * kChunk;
     const int64_t left = p.numel[t] - at;
-    const int64_t n = left < kChunk ? left : kChunk;
+    const int n = static_cast<int>(left < kChunk ? left : kChunk);
     if (p.dtype[t] == B200S_BF16)
       a += sumsq_span(static_cast<const __nv_bfloat16*>(p.src[t]) + at, n);
     else if (p.dtype[t] == B200S_FP16)
@@ -104,12 +161,44 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* parts, int
   if (threadIdx.x == 0) *norm_out = static_cast<float>(sqrt(total));
 }
 
+// Vectors of as many elements as fill 16 bytes of the wider type, so that a warp's accesses on both sides
+// are gapless (bf16 to fp32 with 16-byte loads and two stores each: 224 us for 326 + 652 MB).
 template <typename S, typename D>
-__device__ __forceinline__ void scale_span(const S* x, D* y, int64_t n, float c) {
-  for (int64_t i = threadIdx.x; i < n; i += kThreads) y[i] = from_f<D>(to_f(x[i]) * c);
+__device__ __forceinline__ void scale_span(const S* x, D* y, int n, float c) {
+  constexpr int V = sizeof(S) > sizeof(D) ? 16 / sizeof(S) : 16 / sizeof(D);
+  constexpr int B = 64 / (V * sizeof(S));     // 64 bytes a thread on their way
+  int head;
+  if constexpr (sizeof(S) >= sizeof(D))
+    head = head_of(x, n);
+  else
+    head = head_of(y, n);
+  if (reinterpret_cast<uintptr_t>(y + head) % (V * sizeof(D)) != 0 || reinterpret_cast<uintptr_t>(x + head) % (V * sizeof(S)) != 0) {
+    for (int i = threadIdx.x; i < n; i += kThreads) y[i] = from_f<D>(to_f(x[i]) * c);
+    return;
+  }
+  const int vecs = (n - head) / V;
+  const int tail = head + vecs * V;
+  if (static_cast<int>(threadIdx.x) < head) y[threadIdx.x] = from_f<D>(to_f(x[threadIdx.x]) * c);
+  if (tail + static_cast<int>(threadIdx.x) < n) y[tail + threadIdx.x] = from_f<D>(to_f(x[tail + threadIdx.x]) * c);
+  const float2 cc = make_float2(c, c);
+  for (int i = threadIdx.x; i < vecs; i += B * kThreads) {
+    Pack<S, V> v[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (i + b * kThreads < vecs) v[b] = row::ld<Pack<S, V>>(x + head + (i + b * kThreads) * V);
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      if (i + b * kThreads < vecs) {
+        Pack<D, V> o;
+#pragma unroll
+        for (int k = 0; k < V / 2; ++k) row::store2(o.e + 2 * k, row::mul_(row::load2(v[b].e + 2 * k), cc));
+        row::st(y + head + (i + b * kThreads) * V, o);
+      }
+    }
+  }
 }
 template <typename S>
-__device__ __forceinline__ void scale_to(const S* x, void* dst, int dst_dtype, int64_t at, int64_t n, float c) {
+__device__ __forceinline__ void scale_to(const S* x, void* dst, int dst_dtype, int64_t at, int n, float c) {
   if (dst_dtype == B200S_BF16)
     scale_span(x, static_cast<__nv_bfloat16*>(dst) + at, n, c);
   else if (dst_dtype == B200S_FP16)
@@ -120,7 +209,10 @@ __device__ __forceinline__ void scale_to(const S* x, void* dst, int dst_dtype, i
 
 // Every block forms the same norm from the parts, then scales its chunks. A coefficient of 1 leaves
 // tensors that are clipped in place untouched; a NaN norm makes the coefficient, and them, NaN.
-__global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ ListParams p, const double* parts, int n_parts,
+// S and D are the types of a list whose tensors all go from one to the other, void for any other list. (With all
+// nine pairs in one kernel the spans take 255 registers, or spill: 220 .. 290 us for 326 MB of bf16 to fp32.)
+template <int CAP, typename S, typename D>
+__global__ void __launch_bounds__(kThreads, 5) clip_kernel(const __grid_constant__ ListParams<CAP> p, const double* parts, int n_parts,
                                                         float max_norm, float* norm_out) {
   __shared__ double slots[kThreads / 32];
   const double norm = sqrt(total_of(parts, n_parts, slots));
@@ -128,18 +220,23 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
   const double q = static_cast<double>(max_norm) / (norm + 1e-6);
   const float c = q >= 1. ? 1.f : static_cast<float>(q);
   const int chunks = p.chunk0[p.count];
-  for (int j = blockIdx.x; j < chunks; j += gridDim.x) {
+  for (int k = blockIdx.x; k < chunks; k += gridDim.x) {
+    const int j = chunks - 1 - k;
     const int t = find_tensor(p, j);
     if (c == 1.f && p.dst[t] == p.src[t]) continue;
     const int64_t at = static_cast<int64_t>(j - p.chunk0[t]) * kChunk;
     const int64_t left = p.numel[t] - at;
-    const int64_t n = left < kChunk ? left : kChunk;
-    if (p.dtype[t] == B200S_BF16)
-      scale_to(static_cast<const __nv_bfloat16*>(p.src[t]) + at, p.dst[t], p.dst_dtype[t], at, n, c);
-    else if (p.dtype[t] == B200S_FP16)
-      scale_to(static_cast<const __half*>(p.src[t]) + at, p.dst[t], p.dst_dtype[t], at, n, c);
-    else
-      scale_to(static_cast<const float*>(p.src[t]) + at, p.dst[t], p.dst_dtype[t], at, n, c);
+    const int n = static_cast<int>(left < kChunk ? left : kChunk);
+    if constexpr (!std::is_void_v<S>) {
+      scale_span(static_cast<const S*>(p.src[t]) + at, static_cast<D*>(p.dst[t]) + at, n, c);
+    } else {
+      if (p.dtype[t] == B200S_BF16)
+        scale_to(static_cast<const __nv_bfloat16*>(p.src[t]) + at, p.dst[t], p.dst_dtype[t], at, n, c);
+      else if (p.dtype[t] == B200S_FP16)
+        scale_to(static_cast<const __half*>(p.src[t]) + at, p.dst[t], p.dst_dtype[t], at, n, c);
+      else
+        scale_to(static_cast<const float*>(p.src[t]) + at, p.dst[t], p.dst_dtype[t], at, n, c);
+    }
   }
 }
 
@@ -191,10 +288,11 @@ int check_overlap(const b200s_tensor* list, int64_t count) {
 }
 
 // Takes tensors from list[*next] on until the launch is full; returns the number of chunks.
-int fill(const b200s_tensor* list, int64_t count, int64_t* next, ListParams* p) {
+template <int CAP>
+int fill(const b200s_tensor* list, int64_t count, int64_t* next, ListParams<CAP>* p) {
   p->count = 0;
   int64_t chunks = 0;
-  while (*next < count && p->count < kCapacity) {
+  while (*next < count && p->count < CAP) {
     const b200s_tensor& t = list[*next];
     const int64_t c = (t.numel + kChunk - 1) / kChunk;
     if (chunks + c > INT32_MAX / 2) break;
@@ -208,6 +306,27 @@ int fill(const b200s_tensor* list, int64_t count, int64_t* next, ListParams* p) 
   }
   p->chunk0[p->count] = static_cast<int32_t>(chunks);
   return static_cast<int>(chunks);
+}
+
+// launch(params, blocks' worth of chunks, is it the first) for every launch a list takes.
+template <int CAP, typename F>
+int for_launches(const b200s_tensor* list, int64_t count, F&& launch) {
+  ListParams<CAP> p;
+  int64_t next = 0;
+  bool first = true;
+  do {
+    const int chunks = fill<CAP>(list, count, &next, &p);
+    if (chunks == 0 && !first) break;
+    launch(p, chunks < 1 ? 1 : chunks, first);
+    B200S_CUDA_OK(cudaGetLastError());
+    count_launch();
+    first = false;
+  } while (next < count);
+  return B200S_OK;
+}
+template <typename F>
+int for_launches(const b200s_tensor* list, int64_t count, F&& launch) {
+  return count <= kSmall ? for_launches<kSmall>(list, count, launch) : for_launches<kLarge>(list, count, launch);
 }
 
 }  // namespace
@@ -224,19 +343,10 @@ int b200s_grad_sumsq(const b200s_tensor* list, int64_t count, double* parts, voi
   if (!parts) return B200S_ERR_NULL_POINTER;
   if (!device_status_words()) return B200S_ERR_NO_DEVICE;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  ListParams p;
-  int64_t next = 0;
-  bool first = true;
-  do {
-    int chunks = fill(list, count, &next, &p);
-    if (chunks == 0 && !first) break;
-    const int grid = chunks < 1 ? 1 : (chunks < B200S_NORM_PARTS ? chunks : B200S_NORM_PARTS);
+  return for_launches(list, count, [&](const auto& p, int chunks, bool first) {
+    const int grid = chunks < B200S_NORM_PARTS ? chunks : B200S_NORM_PARTS;
     sumsq_kernel<<<grid, kThreads, 0, s>>>(p, parts, first ? 0 : 1);
-    B200S_CUDA_OK(cudaGetLastError());
-    count_launch();
-    first = false;
-  } while (next < count);
-  return B200S_OK;
+  });
 }
 
 int b200s_grad_norm(const double* parts, int n_parts, float* norm_out, void* stream) {
@@ -259,19 +369,37 @@ int b200s_grad_clip(const b200s_tensor* list, int64_t count, const double* parts
   if (rc) return rc;
   if (!device_status_words()) return B200S_ERR_NO_DEVICE;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  ListParams p;
-  int64_t next = 0;
-  bool first = true;
-  do {
-    int chunks = fill(list, count, &next, &p);
-    if (chunks == 0 && !first) break;
-    const int grid = chunks < 1 ? 1 : (chunks < 148 * 8 ? chunks : 148 * 8);
-    clip_kernel<<<grid, kThreads, 0, s>>>(p, parts, n_parts, max_norm, first ? norm_out : nullptr);
-    B200S_CUDA_OK(cudaGetLastError());
-    count_launch();
-    first = false;
-  } while (next < count);
-  return B200S_OK;
+  return for_launches(list, count, [&](const auto& p, int chunks, bool first) {
+    constexpr int CAP = sizeof(p) > 4096 ? kLarge : kSmall;
+    const int grid = chunks < 148 * 10 ? chunks : 148 * 10;
+    float* norm = first ? norm_out : nullptr;
+    bool same = true;
+    for (int i = 1; i < p.count; ++i) same = same && p.dtype[i] == p.dtype[0] && p.dst_dtype[i] == p.dst_dtype[0];
+    const int pair = same && p.count > 0 ? p.dtype[0] * 3 + p.dst_dtype[0] : -1;
+    using B = __nv_bfloat16;
+    using H = __half;
+    auto go = [&](auto from, auto to) {
+      using S = std::remove_pointer_t<decltype(from)>;
+      using D = std::remove_pointer_t<decltype(to)>;
+      clip_kernel<CAP, S, D><<<grid, kThreads, 0, s>>>(p, parts, n_parts, max_norm, norm);
+    };
+    B* b = nullptr;
+    H* h = nullptr;
+    float* f = nullptr;
+    void* v = nullptr;
+    switch (pair) {
+      case B200S_BF16 * 3 + B200S_BF16: go(b, b); break;
+      case B200S_BF16 * 3 + B200S_FP16: go(b, h); break;
+      case B200S_BF16 * 3 + B200S_FP32: go(b, f); break;
+      case B200S_FP16 * 3 + B200S_BF16: go(h, b); break;
+      case B200S_FP16 * 3 + B200S_FP16: go(h, h); break;
+      case B200S_FP16 * 3 + B200S_FP32: go(h, f); break;
+      case B200S_FP32 * 3 + B200S_BF16: go(f, b); break;
+      case B200S_FP32 * 3 + B200S_FP16: go(f, h); break;
+      case B200S_FP32 * 3 + B200S_FP32: go(f, f); break;
+      default: go(v, v);
+    }
+  });
 }
 
 }  // extern "C"

@@ -177,7 +177,7 @@ __device__ __forceinline__ void ld_params(const void* p, int c, float fill, Pack
     constexpr int N = VEC * sizeof(W) > 16 ? 16 / sizeof(W) : VEC;   // elements of one access
 #pragma unroll
     for (int k = 0; k < VEC; k += N)
-      *reinterpret_cast<Pack<W, N>*>(out.e + k) = *reinterpret_cast<const Pack<W, N>*>(static_cast<const W*>(p) + c + k);
+      *reinterpret_cast<Pack<W, N>*>(out.e + k) = row::ld_const<Pack<W, N>>(static_cast<const W*>(p) + c + k);
   } else {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) out.e[k] = from_f<W>(fill);
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(TH == 32 ? 32 * kWarpRows : TH) norm_fwd_kerne
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * width + lane) * VEC;
-      if (c < d) next[i] = *reinterpret_cast<const P*>(x + c);
+      if (c < d) next[i] = row::ld_const<P>(x + c);
     }
   };
   if (first < p.rows) fetch(first);
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(TH == 32 ? 32 * kWarpRows : TH) norm_fwd_kerne
 #pragma unroll
         for (int k = 0; k < U::count; ++k)
           row::set_unit<T, VEC>(out, k, fma_(mul_(x[i][k], scale), row::unit_of<W, VEC>(w, k), row::unit_of<W, VEC>(b, k)));
-        *reinterpret_cast<P*>(y + c) = out;
+        row::st(y + c, out);
       }
     }
     if (lane == 0 && p.mean) {
@@ -372,8 +372,8 @@ norm_bwd_kernel(const NormBwd p) {
     for (int i = 0; i < NV; ++i) {
       const int c = (i * width + lane) * VEC;
       if (c < d) {
-        xd[i] = *reinterpret_cast<const P*>(x + c);
-        gd[i] = *reinterpret_cast<const P*>(g + c);
+        xd[i] = row::ld_const<P>(x + c);
+        gd[i] = row::ld_const<P>(g + c);
       }
     }
     m = p.mean[r];
@@ -441,7 +441,7 @@ norm_bwd_kernel(const NormBwd p) {
             const F g = mul_(row::unit_of<T, VEC>(gc[i], k), row::unit_of<W, VEC>(w, k));
             row::set_unit<T, VEC>(out, k, fma_(g, scale, fma_(xh, m2, m1)));
           }
-          *reinterpret_cast<P*>(dx + c) = out;
+          row::st(dx + c, out);
         }
       }
     }
@@ -576,7 +576,7 @@ norm_fwd_ring_kernel(const NormFwd p, int stages, uint32_t* status) {
     for (int i = 0; i < NV; ++i) {
       const int c = static_cast<int>(i * TH + threadIdx.x) * VEC;
       if (c < d) {
-        const P v = *reinterpret_cast<const P*>(rowp + c * sizeof(T));
+        const P v = row::ld<P>(rowp + c * sizeof(T));
 #pragma unroll
         for (int k = 0; k < U::count; ++k) {
           x[i][k] = row::unit_of<T, VEC>(v, k);
@@ -622,7 +622,7 @@ norm_fwd_ring_kernel(const NormFwd p, int stages, uint32_t* status) {
 #pragma unroll
         for (int k = 0; k < U::count; ++k)
           row::set_unit<T, VEC>(out, k, fma_(mul_(x[i][k], scale), row::unit_of<W, VEC>(w, k), row::unit_of<W, VEC>(b, k)));
-        *reinterpret_cast<P*>(y + c) = out;
+        row::st(y + c, out);
       }
     }
     if (threadIdx.x == 0 && p.mean) {
@@ -685,8 +685,8 @@ norm_bwd_ring_kernel(const NormBwd p, int stages, uint32_t* status) {
     for (int i = 0; i < NV; ++i) {
       const int c = static_cast<int>(i * TH + threadIdx.x) * VEC;
       if (c < d) {
-        xc[i] = *reinterpret_cast<const P*>(rowp + c * sizeof(T));
-        gc[i] = *reinterpret_cast<const P*>(rowp + row_bytes + c * sizeof(T));
+        xc[i] = row::ld<P>(rowp + c * sizeof(T));
+        gc[i] = row::ld<P>(rowp + row_bytes + c * sizeof(T));
         Pack<W, VEC> w;
         if constexpr (kKeep)
           w = kw[i];
@@ -731,7 +731,7 @@ norm_bwd_ring_kernel(const NormBwd p, int stages, uint32_t* status) {
             const F g = mul_(row::unit_of<T, VEC>(gc[i], k), row::unit_of<W, VEC>(w, k));
             row::set_unit<T, VEC>(out, k, fma_(g, scale, fma_(xh, m2, m1)));
           }
-          *reinterpret_cast<P*>(dx + c) = out;
+          row::st(dx + c, out);
         }
       }
     }

@@ -351,13 +351,13 @@ __global__ void __launch_bounds__(kThreads, 5) logprob_fwd_kernel(const LogprobF
     for (; i + (B - 1) * kThreads < v1; i += B * kThreads) {
       Pack<T, V> v[B];
 #pragma unroll
-      for (int b = 0; b < B; ++b) v[b] = body[i + b * kThreads];
+      for (int b = 0; b < B; ++b) v[b] = row::ld_const<Pack<T, V>>(body + i + b * kThreads);
       add_batch<T, ENT, B>(a, v, s2, u2);
     }
     if (v1 - v0 >= 4 * B * kThreads) {
       // what is left of a long part: a few vectors, one by one
       for (; i < v1; i += kThreads) {
-        const Pack<T, V> v[1] = {body[i]};
+        const Pack<T, V> v[1] = {row::ld_const<Pack<T, V>>(body + i)};
         add_batch<T, ENT, 1>(a, v, s2, u2);
       }
     } else if (i < v1) {
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 5) logprob_fwd_kernel(const LogprobF
 #pragma unroll
       for (int b = 0; b < B; ++b) {
         if (i + b * kThreads < v1) {
-          v[b] = body[i + b * kThreads];
+          v[b] = row::ld_const<Pack<T, V>>(body + i + b * kThreads);
         } else {
 #pragma unroll
           for (int e = 0; e < V; ++e) v[b].e[e] = from_f<T>(kNegInf);
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobBwd 
     const int c = sp.head + i * V;
     P out;
     if (c + V <= limit) {
-      const P v = *reinterpret_cast<const P*>(x + c);
+      const P v = row::ld<P>(x + c);
 #pragma unroll
       for (int k = 0; k < V / 2; ++k) {
         const float2 lp = row::add_(row::load2(v.e + 2 * k), sh);
@@ -533,11 +533,11 @@ __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobBwd 
         for (int e = 0; e < V; ++e)
           if (c + e == target) out.e[e] = from_f<T>(w);
       }
-      *reinterpret_cast<P*>(d + c) = out;
+      row::st(d + c, out);
     } else if (c >= limit) {
 #pragma unroll
       for (int e = 0; e < V; ++e) out.e[e] = from_f<T>(0.f);
-      *reinterpret_cast<P*>(d + c) = out;
+      row::st(d + c, out);
     } else {
       for (int e = 0; e < V; ++e) one(c + e);
     }

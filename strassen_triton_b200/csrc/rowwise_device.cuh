@@ -121,6 +121,44 @@ __device__ __forceinline__ void set_unit(Pack<T, VEC>& v, int k, typename Unit<V
     store2(v.e + 2 * k, u);
 }
 
+// One access of a whole vector. (Copying a Pack member by member leaves the width of the access to the
+// compiler, which does not always find it.) ld_const is for data nobody writes during the launch.
+template <int BYTES>
+struct Raw;
+template <>
+struct Raw<16> {
+  using type = uint4;
+};
+template <>
+struct Raw<8> {
+  using type = uint2;
+};
+template <>
+struct Raw<4> {
+  using type = uint32_t;
+};
+template <>
+struct Raw<2> {
+  using type = unsigned short;
+};
+template <typename P>
+__device__ __forceinline__ P ld(const void* p) {
+  using R = typename Raw<sizeof(P)>::type;
+  const R q = *static_cast<const R*>(p);
+  return *reinterpret_cast<const P*>(&q);
+}
+template <typename P>
+__device__ __forceinline__ P ld_const(const void* p) {
+  using R = typename Raw<sizeof(P)>::type;
+  const R q = __ldg(static_cast<const R*>(p));
+  return *reinterpret_cast<const P*>(&q);
+}
+template <typename P>
+__device__ __forceinline__ void st(void* p, const P& v) {
+  using R = typename Raw<sizeof(P)>::type;
+  *static_cast<R*>(p) = *reinterpret_cast<const R*>(&v);
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

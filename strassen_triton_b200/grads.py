@@ -1,13 +1,14 @@
 """The global gradient norm over many tensors and clipping to it: `grad_norm`, `clip_grads_` on a list of
 gradients, `clip_grad_norm_` on parameters (torch.nn.utils' name and formula).
 
-Two launches for a whole model (every 128 tensors), no synchronisation, no copy of the gradients: the
+Two launches for a whole model (more for lists of over 512 tensors), no synchronisation, no copy of the gradients: the
 sum of squares (in fp64), then one pass that forms the coefficient on the device and scales. When the
 norm is below the bound that pass reads and writes nothing.
 """
 from __future__ import annotations
 
 import math
+from array import array
 from typing import Iterable, Optional, Sequence
 
 import torch
@@ -31,33 +32,49 @@ def _dense(t: Tensor) -> bool:
     return True
 
 
-def _checked(grads: Sequence[Tensor], what: str):
+def _checked(grads: Sequence[Tensor], what: str) -> torch.device:
+    """The device of a list of tensors the kernels can take; raises for anything else."""
     if not grads:
         raise ValueError(f"{what} is empty")
-    dev = grads[0].device if isinstance(grads[0], Tensor) else None
     for t in grads:
-        if not isinstance(t, Tensor) or not t.is_cuda or t.device != dev:
-            require_cuda(grads[0], t)
+        require_cuda(grads[0], t)
         if t.dtype not in DTYPE:
             raise TypeError(f"unsupported dtype {t.dtype} in {what} (bfloat16, float16 and float32 are supported)")
         if t.layout is not torch.strided:
             raise TypeError(f"{what} must hold dense tensors")
-    return dev
+    return grads[0].device
+
+
+def _plain_words(grads):
+    """The entries of a list whose tensors are all contiguous, of supported types and on one GPU (what gradients
+    nearly always are), in one quick pass; None for any other list."""
+    words, dev = [], -1
+    get = DTYPE.get
+    try:
+        for t in grads:
+            code, d = get(t.dtype), t.get_device()
+            if code is None or d < 0 or (d != dev and words) or t.layout is not torch.strided or not t.is_contiguous():
+                return None
+            dev = d
+            p = t.data_ptr()
+            words += (p, p, t.numel(), code | code << 32)
+    except AttributeError:
+        return None
+    return words or None
 
 
 def _entries(src, dst):
-    n = len(src)
-    arr = (_lib.TensorEntry * n)()
-    for e, s, d in zip(arr, src, dst):
-        e.src, e.dst, e.numel = s.data_ptr(), d.data_ptr(), s.numel()
-        e.dtype, e.dst_dtype = DTYPE[s.dtype], DTYPE[d.dtype]
-    return arr
+    """An array of struct b200s_tensor: four 64-bit words each, the two types in the last."""
+    words = []
+    for s, d in zip(src, dst):
+        words += (s.data_ptr(), d.data_ptr(), s.numel(), DTYPE[s.dtype] | DTYPE[d.dtype] << 32)
+    return array("q", words)
 
 
 def _sumsq(dev, arr, n, group):
     """(parts, how many of them count): the partial sums of squares, of all ranks of ``group`` when given."""
     parts = torch.empty(_lib.NORM_PARTS, dtype=torch.float64, device=dev)
-    call(dev, _lib.load().b200s_grad_sumsq, arr, n, parts.data_ptr())
+    call(dev, _lib.load().b200s_grad_sumsq, arr.buffer_info()[0], n, parts.data_ptr())
     if group is None:
         return parts, _lib.NORM_PARTS
     import torch.distributed as dist
@@ -71,9 +88,14 @@ def grad_norm(grads: Iterable[Tensor], *, group=None) -> Tensor:
     """sqrt of the sum of squares over all tensors, a 0-d float32 tensor, on the current stream. ``group``: a
     process group whose ranks each hold a shard of the gradients; their sums of squares are added."""
     grads = list(grads)
-    dev = _checked(grads, "grads")
-    flat = [t if _dense(t) else t.contiguous() for t in grads]
-    parts, n_parts = _sumsq(dev, _entries(flat, flat), len(flat), group)
+    words = _plain_words(grads)
+    if words is not None:
+        dev, arr = grads[0].device, array("q", words)
+    else:
+        dev = _checked(grads, "grads")
+        grads = [t if _dense(t) else t.contiguous() for t in grads]
+        arr = _entries(grads, grads)
+    parts, n_parts = _sumsq(dev, arr, len(grads), group)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     call(dev, _lib.load().b200s_grad_norm, parts.data_ptr(), n_parts, norm.data_ptr())
     return norm
@@ -90,46 +112,59 @@ def clip_grads_(grads: Iterable[Tensor], max_norm: float, *, out: Optional[Seque
     makes all results NaN, unless ``error_if_nonfinite`` (which waits for the GPU) raises first. ``group`` as in
     `grad_norm`. A tensor that is written may appear only once and overlap no other one."""
     grads = list(grads)
-    dev = _checked(grads, "grads")
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0:
         raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
-    src = [t if _dense(t) else t.contiguous() for t in grads]
+    words = _plain_words(grads)
+    dev = grads[0].device if words is not None else _checked(grads, "grads")
+    src, back = grads, []
+    if words is None:
+        src = [t if _dense(t) else t.contiguous() for t in grads]
     if out is None:
-        for t in grads:
-            if any(st == 0 and sz > 1 for sz, st in zip(t.shape, t.stride())):
-                raise ValueError("a gradient with repeated elements (an expanded tensor) cannot be scaled in place")
-        dst, back = src, [(t, s) for t, s in zip(grads, src) if t is not s]
+        if words is None:
+            for t in grads:
+                if any(st == 0 and sz > 1 for sz, st in zip(t.shape, t.stride())):
+                    raise ValueError("a gradient with repeated elements (an expanded tensor) cannot be scaled in place")
+            back = [(t, s) for t, s in zip(grads, src) if t is not s]
+            words = _entries(src, src)
+        arr = array("q", words)
     else:
         out = list(out)
         if len(out) != len(grads):
             raise ValueError(f"out holds {len(out)} tensors for {len(grads)} gradients")
-        _checked(out, "out")
+        quick = _plain_words(out) if words is not None else None
+        if quick is None:
+            _checked(out, "out")
         if out[0].device != dev:
             raise ValueError(f"tensors on different devices: {dev} and {out[0].device}")
-        dst, back = [], []
         for i, (t, o) in enumerate(zip(grads, out)):
             if o.shape != t.shape:
                 raise ValueError(f"out[{i}] has shape {tuple(o.shape)}, its gradient {tuple(t.shape)}")
-            if o.is_contiguous():
-                if not src[i].is_contiguous():
+        if quick is not None:
+            words[1::4] = quick[1::4]
+            words[3::4] = [a & 0xffffffff | b & ~0xffffffff for a, b in zip(words[3::4], quick[3::4])]
+            arr = array("q", words)
+        else:
+            src, dst = list(src), []
+            for i, o in enumerate(out):
+                if o.is_contiguous():
                     src[i] = src[i].contiguous()
-                dst.append(o)
-            elif o.stride() == src[i].stride():
-                dst.append(o)
-            else:
-                src[i] = src[i].contiguous()
-                dst.append(torch.empty(o.shape, dtype=o.dtype, device=dev))
-                back.append((o, dst[-1]))
+                    dst.append(o)
+                elif o.stride() == src[i].stride() and _dense(o):
+                    dst.append(o)
+                else:
+                    src[i] = src[i].contiguous()
+                    dst.append(torch.empty(o.shape, dtype=o.dtype, device=dev))
+                    back.append((o, dst[-1]))
+            arr = _entries(src, dst)
     lib = _lib.load()
-    arr = _entries(src, dst)
-    parts, n_parts = _sumsq(dev, arr, len(src), group)
+    parts, n_parts = _sumsq(dev, arr, len(grads), group)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     if error_if_nonfinite:
         call(dev, lib.b200s_grad_norm, parts.data_ptr(), n_parts, norm.data_ptr())
         if not math.isfinite(norm.item()):
             raise RuntimeError("the norm of the gradients is not finite, so they cannot be clipped")
-    call(dev, lib.b200s_grad_clip, arr, len(src), parts.data_ptr(), n_parts, max_norm, norm.data_ptr())
+    call(dev, lib.b200s_grad_clip, arr.buffer_info()[0], len(grads), parts.data_ptr(), n_parts, max_norm, norm.data_ptr())
     for t, s in back:
         t.copy_(s)
     return norm
