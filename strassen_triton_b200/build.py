@@ -15,7 +15,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(os.path.dirname(PKG_DIR), "include")
 LIB_PATH = os.path.join(PKG_DIR, "libb200s.so")
 SOURCES = ["api.cu", "gemm_sm100.cu", "preadd.cu", "combine.cu", "transpose.cu", "peer.cu",
-           "epilogue.cu", "layernorm.cu", "logprobs.cu", "gradnorm.cu"]
+           "epilogue.cu", "linear_sm100.cu", "layernorm.cu", "logprobs.cu", "gradnorm.cu"]
 
 
 def _nvcc() -> str:

@@ -71,6 +71,35 @@ int launch_gemm(const GemmArgs& g, cudaStream_t stream);
 // device status words (the self-test behind b200s_wait_probe).
 int launch_wait_probe(uint64_t limit_ns, cudaStream_t stream);
 
+// Tensor map (a CUtensorMap at `map`) over an operand stored as [batch][rows][cols], cols contiguous, with a
+// box of box_rows x 128 bytes and the 128-byte swizzle.
+int encode_operand_map(void* map, const void* ptr, int dtype, int64_t rows, int64_t cols, int64_t ld, int64_t batch,
+                       int64_t batch_stride, int box_rows, bool for_store);
+
+// ---- linear layer with its epilogue (linear_sm100.cu) --------------------------------------
+// z = A . B + bias, C = act(z) + residual on 16-bit operands and results, one product. Leading dimensions in
+// elements. `partials` receives splits x M x ldp fp32 partial products instead when splits > 1.
+struct LinearArgs {
+  const void* A;
+  const void* B;
+  void* C;
+  const void* bias;
+  const void* residual;
+  void* preact;
+  float* partials;
+  int64_t M, N, K;
+  int64_t lda, ldb, ldc, ldr, ldz, ldp;
+  int a_major, b_major, in_dtype, out_dtype, activation;
+};
+// How a product is computed, by its extents and majors alone.
+struct LinearPlan {
+  enum Kind { kSkinny, kTiles } kind;
+  int cta_group, tile_n;   // of the tile kernel
+  int splits;              // parts K is cut into (1: the epilogue runs in the product's kernel)
+};
+LinearPlan plan_linear(int64_t M, int64_t N, int64_t K, int a_major, int b_major);
+int launch_linear(const LinearArgs& g, const LinearPlan& plan, cudaStream_t stream);
+
 // ---- fused Strassen kernel (gemm_sm100.cu) ------------------------------------------------
 // One persistent launch that runs the grouped product over all 7^depth operand blocks while four
 // extra warps per CTA ("adders") form the operand blocks of the later outer groups and recombine

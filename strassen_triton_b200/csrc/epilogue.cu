@@ -4,9 +4,10 @@
 //   z = A . B + bias,  C = act(z) + residual                     (b200s_matmul_epilogue)
 //   dz = dy * act'(z),  dbias = sum over rows of dz               (b200s_epilogue_backward)
 //
-// This file holds the forms that work for every product b200s_matmul takes: the product goes to fp32
-// scratch, one pass adds the bias, applies the activation, adds the residual and rounds once. The
-// pre-activation z the backward pass needs is stored in the type of C.
+// A dense product of 16-bit operands and results runs its epilogue inside the product's kernel
+// (linear_sm100.cu). For every other product b200s_matmul takes (fp32, Strassen), and where K is cut into
+// parts, fp32 products go to scratch and one pass here adds them up, adds the bias, applies the activation,
+// adds the residual and rounds once. The pre-activation z the backward pass needs is stored in the type of C.
 
 #include <cuda_runtime.h>
 
@@ -23,29 +24,68 @@ using row::to_f;
 
 constexpr int kThreads = 256;
 
+using row::Pack;
+
+template <typename T, int ACT>
+__device__ __forceinline__ float act_of(float z) {
+  if constexpr (sizeof(T) == 2)
+    return epi::act_fast<ACT>(z);
+  else
+    return epi::act<ACT>(z);
+}
+template <typename T, int ACT>
+__device__ __forceinline__ float dact_of(float z) {
+  if constexpr (sizeof(T) == 2)
+    return epi::dact_fast<ACT>(z);
+  else
+    return epi::dact<ACT>(z);
+}
+
 struct EpiloguePass {
-  const float* z;          // parts x M x N fp32 partial products
+  const float* z;          // parts x M x ld fp32 partial products
   const void* bias;
   const void* residual;
   void* C;
   void* preact;
-  int64_t M, N, ldr, ldc, ldp;
+  int64_t M, N, ld, ldr, ldc, ldp;
   int parts;
 };
 
-template <typename T, int ACT>
+// VEC columns of a row per thread and step: bound by reading the partial products.
+template <typename T, int ACT, int VEC>
 __global__ void __launch_bounds__(kThreads) epilogue_kernel(const EpiloguePass p) {
-  const int64_t total = p.M * p.N;
+  using F = Pack<float, VEC>;
+  using P = Pack<T, VEC>;
+  const int64_t cols = (p.N + VEC - 1) / VEC, total = p.M * cols, stride = p.M * p.ld;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t r = i / p.N, c = i - r * p.N;
-    float z = p.z[i];
-    for (int k = 1; k < p.parts; ++k) z += p.z[k * total + i];
-    if (p.bias) z += to_f(static_cast<const T*>(p.bias)[c]);
-    if (p.preact) static_cast<T*>(p.preact)[r * p.ldp + c] = from_f<T>(z);
-    float y = epi::act<ACT>(z);
-    if (p.residual) y += to_f(static_cast<const T*>(p.residual)[r * p.ldr + c]);
-    static_cast<T*>(p.C)[r * p.ldc + c] = from_f<T>(y);
+    const int64_t r = i / cols, c = (i - r * cols) * VEC;
+    const float* at = p.z + r * p.ld + c;
+    F z = row::ld<F>(at);
+    for (int k = 1; k < p.parts; ++k) {
+      const F q = row::ld<F>(at + k * stride);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) z.e[e] += q.e[e];
+    }
+    P out;
+    if (p.bias) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) z.e[e] += to_f(static_cast<const T*>(p.bias)[c + e]);
+    }
+    if (p.preact) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) out.e[e] = from_f<T>(z.e[e]);
+      row::st(static_cast<T*>(p.preact) + r * p.ldp + c, out);
+    }
+    P res;
+    if (p.residual) res = row::ld<P>(static_cast<const T*>(p.residual) + r * p.ldr + c);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float y = act_of<T, ACT>(z.e[e]);
+      if (p.residual) y += to_f(res.e[e]);
+      out.e[e] = from_f<T>(y);
+    }
+    row::st(static_cast<T*>(p.C) + r * p.ldc + c, out);
   }
 }
 
@@ -58,52 +98,92 @@ struct EpilogueBwd {
   int slices;
 };
 
-// 32 columns per block; a slice takes rows slice * 8 + ty, + slices * 8, ...
-template <typename T, int ACT>
+// 32 VEC columns per block, 8 rows at a time; a slice takes rows slice * 8 + warp, + slices * 8, ... Columns stay
+// with their thread, so the sums of dz add up in registers, unrounded. Reads z and dy, writes dz: bound by memory.
+template <typename T, int ACT, int VEC>
 __global__ void __launch_bounds__(kThreads) epilogue_bwd_kernel(const EpilogueBwd p) {
-  __shared__ float sb[8][33];
+  using P = Pack<T, VEC>;
+  constexpr int R = VEC == 8 ? 2 : 4;      // rows on their way per thread
+  __shared__ float sb[8][32 * VEC + 1];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + tx;
-  float a = 0.f;
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + tx) * VEC;
+  const int64_t step = static_cast<int64_t>(p.slices) * 8;
+  float a[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) a[e] = 0.f;
   if (c < p.N) {
-    for (int64_t r = static_cast<int64_t>(blockIdx.y) * 8 + ty; r < p.M; r += static_cast<int64_t>(p.slices) * 8) {
-      float g = to_f(static_cast<const T*>(p.dy)[r * p.ldy + c]);
-      if constexpr (ACT != B200S_ACT_NONE) g *= epi::dact<ACT>(to_f(static_cast<const T*>(p.z)[r * p.ldz + c]));
-      if (p.dz) static_cast<T*>(p.dz)[r * p.lddz + c] = from_f<T>(g);
-      a += g;
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.y) * 8 + ty; r0 < p.M; r0 += R * step) {
+      P g[R], z[R];
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const int64_t r = r0 + k * step;
+        if (r < p.M) {
+          g[k] = row::ld<P>(static_cast<const T*>(p.dy) + r * p.ldy + c);
+          if constexpr (ACT != B200S_ACT_NONE) z[k] = row::ld<P>(static_cast<const T*>(p.z) + r * p.ldz + c);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const int64_t r = r0 + k * step;
+        if (r < p.M) {
+          P out;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            float v = to_f(g[k].e[e]);
+            if constexpr (ACT != B200S_ACT_NONE) v *= dact_of<T, ACT>(to_f(z[k].e[e]));
+            a[e] += v;
+            out.e[e] = from_f<T>(v);
+          }
+          if (p.dz) row::st(static_cast<T*>(p.dz) + r * p.lddz + c, out);
+        }
+      }
     }
   }
   if (!p.part) return;
-  sb[ty][tx] = a;
-  __syncthreads();
-  if (ty == 0 && c < p.N) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) a += sb[k][tx];
-    p.part[blockIdx.y * p.N + c] = a;
+  for (int e = 0; e < VEC; ++e) sb[ty][tx * VEC + e] = a[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * VEC; i += kThreads) {
+    const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 * VEC + i;
+    if (col >= p.N) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += sb[k][i];
+    p.part[blockIdx.y * p.N + col] = s;
   }
 }
 
-__global__ void __launch_bounds__(kThreads) column_sum_kernel(const float* part, void* out, int64_t n, int slices, int dtype) {
-  __shared__ float s[8][33];
+constexpr int kSumThreads = 1024;
+__global__ void __launch_bounds__(kSumThreads) column_sum_kernel(const float* part, void* out, int64_t n, int slices, int dtype) {
+  __shared__ float s[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + tx;
   float a = 0.f;
-  if (c < n)
-    for (int k = ty; k < slices; k += 8) a += part[static_cast<int64_t>(k) * n + c];
+  if (c < n) {
+#pragma unroll 8
+    for (int k = ty; k < slices; k += 32) a += part[static_cast<int64_t>(k) * n + c];
+  }
   s[ty][tx] = a;
   __syncthreads();
   if (ty == 0 && c < n) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) a += s[k][tx];
+    for (int k = 1; k < 32; ++k) a += s[k][tx];
     row::st_any(out, dtype, c, a);
   }
 }
 
 bool known_dtype(int d) { return d == B200S_BF16 || d == B200S_FP16 || d == B200S_FP32; }
 
-int bwd_slices(int64_t M) {
-  const int64_t want = (M + 63) / 64;
-  return static_cast<int>(want < 1 ? 1 : (want > 128 ? 128 : want));
+// Slices of the rows: enough blocks for every SM to hold several, at least 16 rows each.
+int bwd_slices(int64_t M, int64_t N) {
+  const int64_t cols = (N + 255) / 256;
+  int64_t want = (148 * 6 + cols - 1) / cols;
+  if (want > (M + 15) / 16) want = (M + 15) / 16;
+  return static_cast<int>(want < 1 ? 1 : (want > 256 ? 256 : want));
+}
+
+bool aligned(const void* p, int64_t ld, int64_t rows, size_t es, size_t to) {
+  return reinterpret_cast<uintptr_t>(p) % to == 0 && (rows <= 1 || (static_cast<size_t>(ld) * es) % to == 0);
 }
 
 template <typename F>
@@ -138,6 +218,39 @@ b200s_problem scratch_product(const b200s_problem* p) {
   return q;
 }
 
+// Does the product run with its epilogue in linear_sm100.cu?
+int in_kernel(const b200s_problem* p, bool* yes) {
+  int32_t algo = 0, depth = 0;
+  int rc = b200s_resolve(p, &algo, &depth);
+  if (rc) return rc;
+  *yes = depth == 0 && dtype_size(p->in_dtype) == 2 && p->out_dtype == p->in_dtype && p->tile_variant == 0;
+  return B200S_OK;
+}
+
+int64_t partial_ld(int64_t N) { return (N + 3) / 4 * 4; }
+
+int run_pass(const EpiloguePass& ep, int dtype, int activation, cudaStream_t stream) {
+  return by_dtype(dtype, [&](auto t) {
+    return epi::by_activation(activation, [&](auto a) -> int {
+      using T = decltype(t);
+      constexpr int ACT = decltype(a)::value;
+      const size_t to = 4 * sizeof(T);
+      const bool vec = ep.N % 4 == 0 && aligned(ep.z, ep.ld, ep.M, 4, 16) && aligned(ep.C, ep.ldc, ep.M, sizeof(T), to) &&
+                       (!ep.preact || aligned(ep.preact, ep.ldp, ep.M, sizeof(T), to)) &&
+                       (!ep.residual || aligned(ep.residual, ep.ldr, ep.M, sizeof(T), to));
+      const int64_t blocks = (ep.M * (vec ? ep.N / 4 : ep.N) + kThreads - 1) / kThreads;
+      const unsigned grid = static_cast<unsigned>(blocks < 148 * 32 ? blocks : 148 * 32);
+      if (vec)
+        epilogue_kernel<T, ACT, 4><<<grid, kThreads, 0, stream>>>(ep);
+      else
+        epilogue_kernel<T, ACT, 1><<<grid, kThreads, 0, stream>>>(ep);
+      B200S_CUDA_OK(cudaGetLastError());
+      count_launch();
+      return B200S_OK;
+    });
+  });
+}
+
 }  // namespace
 
 }  // namespace b200s
@@ -150,6 +263,14 @@ int b200s_matmul_epilogue_workspace(const b200s_problem* p, const b200s_epilogue
   if (!bytes_out) return B200S_ERR_NULL_POINTER;
   int rc = check_epilogue(p, e);
   if (rc) return rc;
+  bool fused = false;
+  rc = in_kernel(p, &fused);
+  if (rc) return rc;
+  if (fused) {
+    const LinearPlan plan = plan_linear(p->M, p->N, p->K, p->a_major, p->b_major);
+    *bytes_out = plan.splits > 1 ? static_cast<size_t>(plan.splits) * static_cast<size_t>(p->M) * static_cast<size_t>(partial_ld(p->N)) * 4 : 0;
+    return B200S_OK;
+  }
   const b200s_problem q = scratch_product(p);
   size_t need = 0;
   rc = b200s_workspace_bytes(&q, &need);
@@ -159,7 +280,7 @@ int b200s_matmul_epilogue_workspace(const b200s_problem* p, const b200s_epilogue
 }
 
 int b200s_matmul_epilogue(const b200s_problem* p, const b200s_epilogue* e, const void* A, const void* B, void* C,
-                          void* workspace, size_t workspace_bytes, void* stream) {
+                          void* workspace, size_t workspace_bytes, void* stream_v) {
   size_t need = 0;
   int rc = b200s_matmul_epilogue_workspace(p, e, &need);
   if (rc) return rc;
@@ -169,28 +290,33 @@ int b200s_matmul_epilogue(const b200s_problem* p, const b200s_epilogue* e, const
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return B200S_ERR_BAD_ALIGNMENT;
   if (reinterpret_cast<uintptr_t>(C) % dtype_size(p->out_dtype)) return B200S_ERR_BAD_ALIGNMENT;
   if (!device_status_words()) return B200S_ERR_NO_DEVICE;
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  bool fused = false;
+  rc = in_kernel(p, &fused);
+  if (rc) return rc;
+  if (fused) {
+    const LinearPlan plan = plan_linear(p->M, p->N, p->K, p->a_major, p->b_major);
+    const int64_t ldp = partial_ld(p->N);
+    const LinearArgs g{A, B, C, e->bias, e->residual, e->preact, static_cast<float*>(workspace), p->M, p->N, p->K,
+                       p->lda, p->ldb, p->ldc, e->ld_residual, e->ld_preact, ldp, p->a_major, p->b_major, p->in_dtype, p->out_dtype, e->activation};
+    rc = launch_linear(g, plan, stream);
+    if (rc || plan.splits == 1) return rc;
+    const EpiloguePass ep{static_cast<const float*>(workspace), e->bias, e->residual, C, e->preact, p->M, p->N, ldp, e->ld_residual, p->ldc, e->ld_preact, plan.splits};
+    return run_pass(ep, p->out_dtype, e->activation, stream);
+  }
   const b200s_problem q = scratch_product(p);
   const size_t zb = round256(static_cast<size_t>(p->M) * static_cast<size_t>(p->N) * 4);
   uint8_t* rest = static_cast<uint8_t*>(workspace) + zb;
-  rc = b200s_matmul(&q, A, B, workspace, need > zb ? rest : nullptr, need - zb, stream);
+  rc = b200s_matmul(&q, A, B, workspace, need > zb ? rest : nullptr, need - zb, stream_v);
   if (rc) return rc;
-  const EpiloguePass ep{static_cast<const float*>(workspace), e->bias, e->residual, C, e->preact, p->M, p->N, e->ld_residual, p->ldc, e->ld_preact, 1};
-  const int64_t blocks = (p->M * p->N + kThreads - 1) / kThreads;
-  const unsigned grid = static_cast<unsigned>(blocks < 148 * 32 ? blocks : 148 * 32);
-  return by_dtype(p->out_dtype, [&](auto t) {
-    return epi::by_activation(e->activation, [&](auto a) -> int {
-      epilogue_kernel<decltype(t), decltype(a)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(ep);
-      B200S_CUDA_OK(cudaGetLastError());
-      count_launch();
-      return B200S_OK;
-    });
-  });
+  const EpiloguePass ep{static_cast<const float*>(workspace), e->bias, e->residual, C, e->preact, p->M, p->N, p->N, e->ld_residual, p->ldc, e->ld_preact, 1};
+  return run_pass(ep, p->out_dtype, e->activation, stream);
 }
 
 int b200s_epilogue_backward_workspace(int64_t M, int64_t N, size_t* bytes_out) {
   if (!bytes_out) return B200S_ERR_NULL_POINTER;
   if (M < 0 || N <= 0 || N > INT32_MAX) return B200S_ERR_BAD_SHAPE;
-  *bytes_out = static_cast<size_t>(bwd_slices(M)) * static_cast<size_t>(N) * sizeof(float);
+  *bytes_out = static_cast<size_t>(bwd_slices(M, N)) * static_cast<size_t>(N) * sizeof(float);
   return B200S_OK;
 }
 
@@ -215,20 +341,33 @@ int b200s_epilogue_backward(int64_t M, int64_t N, int dtype, int activation, con
   }
   if (!device_status_words()) return B200S_ERR_NO_DEVICE;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int slices = bwd_slices(M);
+  const int slices = bwd_slices(M, N);
   float* part = dbias ? static_cast<float*>(workspace) : nullptr;
   const EpilogueBwd b{preact, dy, dz, part, M, N, ldz, ldy, lddz, slices};
-  const unsigned cols = static_cast<unsigned>((N + 31) / 32);
   rc = by_dtype(dtype, [&](auto t) {
-    return epi::by_activation(activation, [&](auto a) -> int {
-      epilogue_bwd_kernel<decltype(t), decltype(a)::value><<<dim3(cols, slices), kThreads, 0, s>>>(b);
+    return epi::by_activation(activation, [&](auto act) -> int {
+      using T = decltype(t);
+      constexpr int ACT = decltype(act)::value;
+      constexpr int W = static_cast<int>(16 / sizeof(T));
+      auto fits = [&](int vec) {
+        const size_t to = vec * sizeof(T);
+        return N % vec == 0 && aligned(dy, ldy, M, sizeof(T), to) && (ACT == B200S_ACT_NONE || aligned(preact, ldz, M, sizeof(T), to)) &&
+               (!dz || aligned(dz, lddz, M, sizeof(T), to));
+      };
+      auto grid = [&](int vec) { return dim3(static_cast<unsigned>((N + 32 * vec - 1) / (32 * vec)), static_cast<unsigned>(slices)); };
+      if (fits(W))
+        epilogue_bwd_kernel<T, ACT, W><<<grid(W), kThreads, 0, s>>>(b);
+      else if (fits(2))
+        epilogue_bwd_kernel<T, ACT, 2><<<grid(2), kThreads, 0, s>>>(b);
+      else
+        epilogue_bwd_kernel<T, ACT, 1><<<grid(1), kThreads, 0, s>>>(b);
       B200S_CUDA_OK(cudaGetLastError());
       count_launch();
       return B200S_OK;
     });
   });
   if (rc || !dbias) return rc;
-  column_sum_kernel<<<cols, kThreads, 0, s>>>(part, dbias, N, slices, dtype);
+  column_sum_kernel<<<static_cast<unsigned>((N + 31) / 32), kSumThreads, 0, s>>>(part, dbias, N, slices, dtype);
   B200S_CUDA_OK(cudaGetLastError());
   count_launch();
   return B200S_OK;

@@ -1109,6 +1109,11 @@ __global__ void __launch_bounds__(32) wait_probe_kernel(uint64_t limit_ns, uint3
 
 }  // namespace
 
+int encode_operand_map(void* map, const void* ptr, int dtype, int64_t rows, int64_t cols, int64_t ld, int64_t batch,
+                       int64_t batch_stride, int box_rows, bool for_store) {
+  return make_operand_map(static_cast<CUtensorMap*>(map), ptr, dtype, rows, cols, ld, batch, batch_stride, box_rows, for_store);
+}
+
 int launch_wait_probe(uint64_t limit_ns, cudaStream_t stream) {
   uint32_t* status = device_status_words();
   if (!status) return B200S_ERR_NO_DEVICE;

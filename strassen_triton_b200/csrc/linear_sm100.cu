@@ -1,0 +1,737 @@
+// Linear layer with its epilogue for sm_100a: z = A . B + bias, C = act(z) + residual, z stored on request.
+// 16-bit operands and results, fp32 accumulation, everything after the product in fp32, one rounding.
+//
+// Two kernels:
+//   linear_kernel   tcgen05 tiles. Warp 0 loads 128-byte-swizzled operand tiles by TMA, one lane of warp 1
+//                   issues tcgen05.mma into one of two accumulators in tensor memory, warps 2..9 take the
+//                   other one through the epilogue: bias, activation, residual, staging in shared memory,
+//                   TMA stores. Tile shapes 256 x 256 and 256 x 128 (CTA pairs), 128 x 128; K may be cut into
+//                   parts whose fp32 partial products a second pass adds up (plan_linear weighs all this).
+//   skinny_kernel   up to 32 rows of A (tokens being generated) against K-major weights: bound by reading the
+//                   weights once, with mma.sync fed straight from global memory in registers.
+//
+// What bounds linear_kernel: tensor cores and the L2 reads of operand tiles; with K below about 1000 the
+// epilogue's arithmetic comes close to the product's (a GELU is 11 instructions and two of the 16-a-clock unit).
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <mutex>
+
+#include "common.h"
+#include "epilogue_device.cuh"
+#include "ptx_sm100.cuh"
+#include "rowwise_device.cuh"
+
+namespace b200s {
+
+namespace {
+
+constexpr int kRowBytes = 128;   // one swizzled row of a tile: 64 elements
+constexpr int kBK = 64;          // K elements per stage
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+
+// Role codes in the status words when a wait runs out.
+enum : uint32_t { kWhoProducer = 13, kWhoMma = 14, kWhoMmaAcc = 15, kWhoEpilogue = 16 };
+constexpr uint64_t kDrainNs = 20ull * 1000 * 1000;
+
+struct LinearParams {
+  int32_t M, N, K;
+  int32_t m_tiles, n_tiles, k_blocks, splits, total_tiles;
+  int32_t raster_group;
+  int32_t a_mn, b_mn, fmt;
+  int32_t bf16_out, act;
+  int32_t tma_c, tma_z;          // results that TMA can store
+  int32_t vec_r;                 // residual rows are 16-byte aligned
+  const void* bias;
+  const void* residual;
+  void* C;
+  void* Z;
+  int64_t ldc, ldr, ldz;
+  uint32_t* status;
+};
+
+struct Tile {
+  int split, mt, nt, kb0, kb1;
+};
+
+__device__ __forceinline__ Tile decode(const LinearParams& p, int tile) {
+  Tile t;
+  const int per = p.m_tiles * p.n_tiles;
+  t.split = tile / per;
+  int r = tile - t.split * per;
+  const int band = p.raster_group * p.n_tiles;
+  const int g = r / band;
+  const int first = g * p.raster_group;
+  const int size = min(p.raster_group, p.m_tiles - first);
+  r -= g * band;
+  t.mt = first + r % size;
+  t.nt = r / size;
+  t.kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * t.split / p.splits);
+  t.kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (t.split + 1) / p.splits);
+  return t;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
+  return bf16 ? ptx::pack_bf16(lo, hi) : ptx::pack_f16(lo, hi);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t u, bool bf16) {
+  return bf16 ? make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+__device__ __forceinline__ float element(const void* p, int64_t i, bool bf16) {
+  return bf16 ? __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + i)) : __half2float(__ldg(static_cast<const __half*>(p) + i));
+}
+
+template <int ACT>
+__device__ __forceinline__ void activate(float (&v)[64]) {
+#pragma unroll
+  for (int j = 0; j < 64; ++j) v[j] = epi::act_fast<ACT>(v[j]);
+}
+__device__ __forceinline__ void activate(float (&v)[64], int act) {
+  switch (act) {      // the same for the whole launch
+    case B200S_ACT_RELU: activate<B200S_ACT_RELU>(v); break;
+    case B200S_ACT_RELU2: activate<B200S_ACT_RELU2>(v); break;
+    case B200S_ACT_SILU: activate<B200S_ACT_SILU>(v); break;
+    case B200S_ACT_GELU: activate<B200S_ACT_GELU>(v); break;
+    case B200S_ACT_GELU_TANH: activate<B200S_ACT_GELU_TANH>(v); break;
+    default: break;
+  }
+}
+
+// One warp's 32 x 64 block of 16-bit results, packed by its lanes (lane = row), goes through a swizzled 4 KB
+// buffer to row0, col0 of a matrix: by TMA, or row by row where TMA cannot address the matrix.
+__device__ __forceinline__ void store_block(const CUtensorMap* map, bool tma, void* dst, int64_t ld, int M, int N, int row0, int col0,
+                                            uint32_t buf, const uint32_t (&h)[32], int lane) {
+  const uint32_t srow = buf + static_cast<uint32_t>(lane) * 128u, sw = static_cast<uint32_t>(lane & 7);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    ptx::st_shared_v4(srow + ((static_cast<uint32_t>(j) ^ sw) << 4), h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+  if (tma) {
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) ptx::tma_store_3d(map, buf, col0, row0, 0);
+    return;
+  }
+  __syncwarp();
+  unsigned short* out = static_cast<unsigned short*>(dst);
+  const int rows = min(32, M - row0), cols = N - col0;
+  for (int r = 0; r < rows; ++r) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int c = lane + 32 * k;
+      uint16_t v;
+      asm volatile("ld.shared.u16 %0, [%1];"
+                   : "=h"(v)
+                   : "r"(buf + static_cast<uint32_t>(r) * 128u + ((static_cast<uint32_t>(c >> 3) ^ static_cast<uint32_t>(r & 7)) << 4) + (c & 7) * 2u));
+      if (c < cols) out[static_cast<int64_t>(row0 + r) * ld + col0 + c] = v;
+    }
+  }
+  __syncwarp();
+}
+
+template <int CG, int BN, int STAGES, bool PARTIAL>
+__global__ void __launch_bounds__(kThreads, 1)
+linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
+              const __grid_constant__ CUtensorMap tmZ, const LinearParams p) {
+  constexpr int BN_CTA = BN / CG;
+  constexpr int A_BYTES = 128 * kRowBytes;
+  constexpr int B_BYTES = BN_CTA * kRowBytes;
+  constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  constexpr int CHUNK_BYTES = kBK * kRowBytes;       // an MN-major chunk: 64 k-rows of 64 elements
+  constexpr int STAGING = kEpiWarps * 2 * 4096;
+  constexpr uint32_t TMEM_COLS = 2 * BN;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const uint32_t staging = base + STAGES * STAGE_BYTES;
+  const uint32_t bars = staging + STAGING;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
+  auto tfull_bar = [&](int b) { return bars + 8u * (2 * STAGES + b); };
+  auto tempty_bar = [&](int b) { return bars + 8u * (2 * STAGES + 2 + b); };
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + STAGES * STAGE_BYTES + STAGING + 8 * (2 * STAGES + 4));
+  volatile uint32_t* abort_word = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? ptx::cluster_ctarank() : 0u;
+  const int cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
+
+  if (threadIdx.x == 0) {
+    *abort_word = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(tfull_bar(b), 1);
+      ptx::mbar_init(tempty_bar(b), kEpiWarps * CG);
+    }
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&tmA);
+    ptx::prefetch_tensormap(&tmB);
+    if (p.tma_c) ptx::prefetch_tensormap(&tmC);
+    if (p.tma_z) ptx::prefetch_tensormap(&tmZ);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<CG>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), TMEM_COLS);
+    ptx::tmem_relinquish<CG>();
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if constexpr (CG == 2) {
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+  }
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      bool alive = true;
+      for (int tile = cluster; alive && tile < p.total_tiles; tile += clusters) {
+        const Tile t = decode(p, tile);
+        const int m0 = t.mt * (128 * CG) + static_cast<int>(rank) * 128;
+        const int n0 = t.nt * BN + static_cast<int>(rank) * BN_CTA;
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          if (!ptx::mbar_wait<CG == 2>(empty_bar(stage), phase ^ 1u, abort_word, kWhoProducer)) {
+            alive = false;
+            break;
+          }
+          const uint32_t sA = base + stage * STAGE_BYTES, sB = sA + A_BYTES;
+          const int k0 = kb * kBK;
+          uint32_t fb = full_bar(stage);
+          if constexpr (CG == 2) fb = ptx::mapa_cluster(fb, 0);
+          if (rank == 0) ptx::mbar_expect_tx(full_bar(stage), CG * STAGE_BYTES);
+          auto load = [&](uint32_t dst, const CUtensorMap* m, int c0, int c1) {
+            if constexpr (CG == 2)
+              ptx::tma_load_3d_pair(dst, m, fb, c0, c1, 0);
+            else
+              ptx::tma_load_3d(dst, m, fb, c0, c1, 0);
+          };
+          if (!p.a_mn) {
+            load(sA, &tmA, k0, m0);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) load(sA + j * CHUNK_BYTES, &tmA, m0 + j * 64, k0);
+          }
+          if (!p.b_mn) {
+            load(sB, &tmB, k0, n0);
+          } else {
+#pragma unroll
+            for (int j = 0; j < BN_CTA / 64; ++j) load(sB + j * CHUNK_BYTES, &tmB, n0 + j * 64, k0);
+          }
+          if (++stage == STAGES) stage = 0, phase ^= 1u;
+        }
+      }
+      if (!alive && rank == 0) {
+        // Copies may still be in flight into this cluster's shared memory: let them land, within a limit.
+        // Stages below `stage` were armed in this pass over the ring, the others in the one before.
+        const uint64_t deadline = ptx::global_timer_ns() + kDrainNs;
+        for (uint32_t s = 0; s < static_cast<uint32_t>(STAGES); ++s)
+          if (!ptx::mbar_wait_until(full_bar(static_cast<int>(s)), s < stage ? phase : phase ^ 1u, deadline)) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = ptx::make_instr_desc(static_cast<uint32_t>(p.fmt), p.a_mn, p.b_mn, 128 * CG, BN);
+      const uint32_t a_lbo = p.a_mn ? CHUNK_BYTES : 16u, b_lbo = p.b_mn ? CHUNK_BYTES : 16u;
+      const uint32_t a_adv = p.a_mn ? 2 * 1024u : 32u, b_adv = p.b_mn ? 2 * 1024u : 32u;
+      const uint64_t a_desc0 = ptx::make_smem_desc(base, a_lbo, 1024u);
+      const uint64_t b_desc0 = ptx::make_smem_desc(base + A_BYTES, b_lbo, 1024u);
+      uint32_t stage = 0, phase = 0;
+      int it = 0;
+      bool alive = true;
+      for (int tile = cluster; alive && tile < p.total_tiles; tile += clusters, ++it) {
+        const Tile t = decode(p, tile);
+        const int buf = it & 1;
+        if (!ptx::mbar_wait<CG == 2>(tempty_bar(buf), ((it >> 1) & 1u) ^ 1u, abort_word, kWhoMmaAcc)) break;
+        ptx::tc_fence_after_sync();
+        const uint32_t acc = tmem + static_cast<uint32_t>(buf * BN);
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          if (!ptx::mbar_wait<CG == 2>(full_bar(stage), phase, abort_word, kWhoMma)) {
+            alive = false;
+            break;
+          }
+          ptx::tc_fence_after_sync();
+          const uint32_t soff = stage * (STAGE_BYTES >> 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            ptx::umma<CG, false>(acc, a_desc0 + (soff + k * (a_adv >> 4)), b_desc0 + (soff + k * (b_adv >> 4)), idesc,
+                                 (kb != t.kb0 || k != 0) ? 1u : 0u);
+          ptx::umma_commit<CG>(empty_bar(stage));
+          if constexpr (CG == 2) ptx::umma_commit<CG>(ptx::mapa_cluster(empty_bar(stage), 1));
+          if (++stage == STAGES) stage = 0, phase ^= 1u;
+        }
+        if (!alive) break;
+        ptx::umma_commit<CG>(tfull_bar(buf));
+        if constexpr (CG == 2) ptx::umma_commit<CG>(ptx::mapa_cluster(tfull_bar(buf), 1));
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int ew = warp - 2;
+    const int lane_group = warp & 3;        // this warp's TMEM lanes [32 * lane_group, +32)
+    const int half = ew >> 2;               // and half of the tile's columns
+    const uint32_t stg = staging + static_cast<uint32_t>(ew) * 8192u;
+    const bool bf16 = p.bf16_out != 0;
+    int flip = 0, it = 0;
+    // the next staging buffer, once the store that last read it is done with it
+    auto next_buffer = [&]() {
+      const uint32_t b = stg + static_cast<uint32_t>(flip) * 4096u;
+      flip ^= 1;
+      if (lane == 0) ptx::tma_store_wait_read<1>();
+      __syncwarp();
+      return b;
+    };
+    auto sent = [&]() {      // every buffer is one bulk group, stored by TMA or not
+      if (lane == 0) ptx::tma_store_commit();
+    };
+    for (int tile = cluster; tile < p.total_tiles; tile += clusters, ++it) {
+      const Tile t = decode(p, tile);
+      const int buf = it & 1;
+      const int row0 = t.mt * (128 * CG) + static_cast<int>(rank) * 128 + lane_group * 32;
+      const int col_first = t.nt * BN + half * (BN / 2);
+      constexpr int GROUPS = BN / 2 / 64;
+      // residual of the first columns: on its way while the product is computed (a row of 64 columns is 8 lanes)
+      uint4 res[8];
+      auto fetch_residual = [&](int col0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = row0 + 4 * i + (lane >> 3), c = col0 + (lane & 7) * 8;
+          res[i] = make_uint4(0, 0, 0, 0);
+          if (r < p.M && c < p.N)
+            res[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) + static_cast<int64_t>(r) * p.ldr + c);
+        }
+      };
+      const bool vec_res = !PARTIAL && p.residual != nullptr && p.vec_r;
+      if (vec_res) fetch_residual(col_first);
+      int ok = 1;
+      if (lane == 0) ok = ptx::mbar_wait<CG == 2, 32>(tfull_bar(buf), (it >> 1) & 1u, abort_word, kWhoEpilogue) ? 1 : 0;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      ptx::tc_fence_after_sync();
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(lane_group * 32) << 16) + static_cast<uint32_t>(buf * BN + half * (BN / 2));
+#pragma unroll 1
+      for (int g = 0; g < GROUPS; ++g) {
+        const int col0 = col_first + g * 64;
+        uint32_t r0[32], r1[32];
+        ptx::tmem_ld_32x32(taddr + g * 64, r0);
+        ptx::tmem_ld_32x32(taddr + g * 64 + 32, r1);
+        ptx::tmem_ld_wait();
+        if (g == GROUPS - 1) {
+          // the accumulator is in registers: the next tile may have it
+          ptx::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 2)
+              ptx::mbar_arrive_cluster(tempty_bar(buf), 0);
+            else
+              ptx::mbar_arrive(tempty_bar(buf));
+          }
+        }
+        if (col0 >= p.N || row0 >= p.M) continue;
+        if constexpr (PARTIAL) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t b = next_buffer();
+            const uint32_t srow = b + static_cast<uint32_t>(lane) * 128u, sw = static_cast<uint32_t>(lane & 7);
+            const uint32_t(&r)[32] = h == 0 ? r0 : r1;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              ptx::st_shared_v4(srow + ((static_cast<uint32_t>(j) ^ sw) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && col0 + 32 * h < p.N) ptx::tma_store_3d(&tmC, b, col0 + 32 * h, row0, t.split);
+            sent();
+          }
+        } else {
+          float v[64];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r0[j]), v[32 + j] = __uint_as_float(r1[j]);
+          if (p.bias != nullptr) {
+            if (col0 + 64 <= p.N && ((reinterpret_cast<uintptr_t>(p.bias) + 2u * static_cast<uintptr_t>(col0)) & 15u) == 0) {
+              const uint4* bp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.bias) + col0);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const uint4 q = __ldg(bp + j);
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const float2 f = unpack2(w[k], bf16);
+                  v[8 * j + 2 * k] += f.x;
+                  v[8 * j + 2 * k + 1] += f.y;
+                }
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 64; ++j)
+                if (col0 + j < p.N) v[j] += element(p.bias, col0 + j, bf16);
+            }
+          }
+          uint32_t h[32];
+          if (p.Z != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) h[j] = pack2(v[2 * j], v[2 * j + 1], bf16);
+            store_block(&tmZ, p.tma_z != 0, p.Z, p.ldz, p.M, p.N, row0, col0, next_buffer(), h, lane);
+            sent();
+          }
+          activate(v, p.act);
+          const uint32_t b = next_buffer();
+          if (p.residual != nullptr) {
+            // rows as they were read -> rows of the lanes, through the buffer the result will use
+            if (vec_res) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t r = static_cast<uint32_t>(4 * i + (lane >> 3)), j = static_cast<uint32_t>(lane & 7);
+                ptx::st_shared_v4(b + r * 128u + ((j ^ (r & 7u)) << 4), res[i].x, res[i].y, res[i].z, res[i].w);
+              }
+              if (g + 1 < GROUPS) fetch_residual(col0 + 64);
+            } else {
+              const int rows = min(32, p.M - row0);
+              for (int r = 0; r < rows; ++r) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const int c = lane + 32 * k;
+                  uint16_t q = 0;
+                  if (col0 + c < p.N) q = static_cast<const uint16_t*>(p.residual)[static_cast<int64_t>(row0 + r) * p.ldr + col0 + c];
+                  asm volatile("st.shared.u16 [%0], %1;" ::"r"(b + static_cast<uint32_t>(r) * 128u +
+                                                               ((static_cast<uint32_t>(c >> 3) ^ static_cast<uint32_t>(r & 7)) << 4) + (c & 7) * 2u),
+                               "h"(q)
+                               : "memory");
+                }
+              }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint4 q = ptx::ld_shared_v4(b + static_cast<uint32_t>(lane) * 128u + ((static_cast<uint32_t>(j) ^ static_cast<uint32_t>(lane & 7)) << 4));
+              const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 f = unpack2(w[k], bf16);
+                v[8 * j + 2 * k] += f.x;
+                v[8 * j + 2 * k + 1] += f.y;
+              }
+            }
+            __syncwarp();
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) h[j] = pack2(v[2 * j], v[2 * j + 1], bf16);
+          store_block(&tmC, p.tma_c != 0, p.C, p.ldc, p.M, p.N, row0, col0, b, h, lane);
+          sent();
+        }
+      }
+    }
+    if (lane == 0) ptx::tma_store_wait_all<0>();     // shared memory must outlive the stores
+    __syncwarp();
+  }
+
+  // ------------------------------------------------------------ teardown
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if constexpr (CG == 2) {
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+  }
+  if (threadIdx.x == 0 && *abort_word != 0) {
+    atomicExch(&p.status[0], 1u);
+    atomicExch(&p.status[1], *abort_word);
+  }
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc<CG>(tmem, TMEM_COLS);
+  }
+}
+
+// ---- few rows of A -------------------------------------------------------------------------------
+// y^T = W x^T with mma.sync m16n8k16: 16 rows of W (outputs) are the A operand, up to 8 * MT rows of x the
+// columns of B. The order of the terms along K is free as long as both operands agree, so lane (g, t) of a
+// warp takes 8 consecutive k of its rows, one 16-byte load, as the fragments of two steps: chunks of 32 k are
+// read whole, 64 bytes a row, without shared memory. The block's 8 warps take every 8th chunk and add up
+// their 16 x 8 MT sums in shared memory.
+constexpr int kSkinnyWarps = 8;
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+struct SkinnyParams {
+  const uint16_t* X;
+  const uint16_t* W;
+  const void* bias;
+  const void* residual;
+  void* C;
+  void* Z;
+  int64_t ldx, ldw, ldc, ldr, ldz;
+  int32_t M, N, K, act;
+};
+
+// 8 elements from column k of a row, zero from column K on (what lies there is not part of the operand).
+__device__ __forceinline__ uint4 row8(const uint16_t* row, int k, int K, bool in) {
+  if (!in || k >= K) return make_uint4(0, 0, 0, 0);
+  uint4 q = __ldg(reinterpret_cast<const uint4*>(row + k));
+  if (k + 8 > K) {
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (k + 2 * j >= K) w[j] = 0;
+      else if (k + 2 * j + 1 >= K) w[j] &= 0xffffu;
+    }
+    q = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return q;
+}
+
+template <int MT, bool BF16>
+__global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const SkinnyParams p) {
+  constexpr int UN = MT <= 2 ? 4 : 2;       // chunks on their way per warp
+  __shared__ float part[kSkinnyWarps][16][8 * MT + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16;
+  const bool in0 = n0 + g < p.N, in1 = n0 + g + 8 < p.N;
+  const uint16_t* w0 = p.W + static_cast<int64_t>(in0 ? n0 + g : 0) * p.ldw;
+  const uint16_t* w1 = p.W + static_cast<int64_t>(in1 ? n0 + g + 8 : 0) * p.ldw;
+  const uint16_t* x[MT];
+  bool inx[MT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    inx[j] = 8 * j + g < p.M;
+    x[j] = p.X + static_cast<int64_t>(inx[j] ? 8 * j + g : 0) * p.ldx;
+  }
+  float acc[MT][4];
+#pragma unroll
+  for (int j = 0; j < MT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+  const int chunks = (p.K + 31) / 32;
+  for (int c = warp; c < chunks; c += kSkinnyWarps * UN) {
+    uint4 a[UN], b[UN], xv[UN][MT];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int k = (c + u * kSkinnyWarps) * 32 + t * 8;
+      a[u] = row8(w0, k, p.K, in0);
+      b[u] = row8(w1, k, p.K, in1);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) xv[u][j] = row8(x[j], k, p.K, inx[j]);
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        mma16816<BF16>(acc[j], a[u].x, b[u].x, a[u].y, b[u].y, xv[u][j].x, xv[u][j].y);
+        mma16816<BF16>(acc[j], a[u].z, b[u].z, a[u].w, b[u].w, xv[u][j].z, xv[u][j].w);
+      }
+  }
+  // accumulator element (row g or g + 8 of W, row 2t or 2t + 1 of x)
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    part[warp][g][8 * j + 2 * t] = acc[j][0];
+    part[warp][g][8 * j + 2 * t + 1] = acc[j][1];
+    part[warp][g + 8][8 * j + 2 * t] = acc[j][2];
+    part[warp][g + 8][8 * j + 2 * t + 1] = acc[j][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * 8 * MT; i += 32 * kSkinnyWarps) {
+    const int n = i & 15, m = i >> 4;
+    if (m >= p.M || n0 + n >= p.N) continue;
+    float z = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSkinnyWarps; ++w) z += part[w][n][m];
+    if (p.bias) z += element(p.bias, n0 + n, BF16);
+    using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    if (p.Z) static_cast<T*>(p.Z)[static_cast<int64_t>(m) * p.ldz + n0 + n] = row::from_f<T>(z);
+    float y = z;
+    switch (p.act) {
+      case B200S_ACT_RELU: y = epi::act_fast<B200S_ACT_RELU>(z); break;
+      case B200S_ACT_RELU2: y = epi::act_fast<B200S_ACT_RELU2>(z); break;
+      case B200S_ACT_SILU: y = epi::act_fast<B200S_ACT_SILU>(z); break;
+      case B200S_ACT_GELU: y = epi::act_fast<B200S_ACT_GELU>(z); break;
+      case B200S_ACT_GELU_TANH: y = epi::act_fast<B200S_ACT_GELU_TANH>(z); break;
+      default: break;
+    }
+    if (p.residual) y += row::to_f(static_cast<const T*>(p.residual)[static_cast<int64_t>(m) * p.ldr + n0 + n]);
+    static_cast<T*>(p.C)[static_cast<int64_t>(m) * p.ldc + n0 + n] = row::from_f<T>(y);
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------------
+
+template <int CG, int BN, int STAGES, bool PARTIAL>
+int launch_tiles(const CUtensorMap* maps, LinearParams p, cudaStream_t stream) {
+  constexpr int SMEM = STAGES * (128 + BN / CG) * kRowBytes + kEpiWarps * 2 * 4096 + 8 * (2 * STAGES + 4) + 16 + 1024;
+  static_assert(SMEM <= 227 * 1024, "shared memory budget");
+  auto kernel = linear_kernel<CG, BN, STAGES, PARTIAL>;
+  static std::mutex mu;
+  static int resident[64] = {0};       // clusters a device holds at once
+  int dev = 0;
+  B200S_CUDA_OK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return B200S_ERR_NO_DEVICE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = SMEM;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int fit;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (resident[dev] == 0) {
+      B200S_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+      int n = sm_count() / CG;
+      if (CG == 2) {
+        cfg.gridDim = dim3(sm_count() / 2 * 2);
+        int q = 0;
+        B200S_CUDA_OK(cudaOccupancyMaxActiveClusters(&q, kernel, &cfg));
+        if (q < 1) return B200S_ERR_CUDA;
+        if (q < n) n = q;
+      }
+      resident[dev] = n;
+    }
+    fit = resident[dev];
+  }
+  const int allowed = product_sm_count() / CG;
+  if (allowed < fit) fit = allowed;
+  if (fit < 1) return B200S_ERR_NO_DEVICE;
+  cfg.gridDim = dim3((p.total_tiles < fit ? p.total_tiles : fit) * CG);
+  cfg.stream = stream;
+  B200S_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], p));
+  count_launch();
+  return B200S_OK;
+}
+
+template <bool PARTIAL>
+int launch_plan(const LinearPlan& plan, const CUtensorMap* maps, const LinearParams& p, cudaStream_t stream) {
+  if (plan.cta_group == 2 && plan.tile_n == 256) return launch_tiles<2, 256, 5, PARTIAL>(maps, p, stream);
+  if (plan.cta_group == 2) return launch_tiles<2, 128, 6, PARTIAL>(maps, p, stream);
+  return launch_tiles<1, 128, 5, PARTIAL>(maps, p, stream);
+}
+
+template <int MT>
+int launch_skinny(const SkinnyParams& p, bool bf16, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>((p.N + 15) / 16);
+  if (bf16)
+    skinny_kernel<MT, true><<<grid, 32 * kSkinnyWarps, 0, stream>>>(p);
+  else
+    skinny_kernel<MT, false><<<grid, 32 * kSkinnyWarps, 0, stream>>>(p);
+  B200S_CUDA_OK(cudaGetLastError());
+  count_launch();
+  return B200S_OK;
+}
+
+bool tma_rows(const void* p, int64_t ld, int64_t rows) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (rows <= 1 || (ld * 2) % 16 == 0);
+}
+
+}  // namespace
+
+LinearPlan plan_linear(int64_t M, int64_t N, int64_t K, int a_major, int b_major) {
+  LinearPlan best{LinearPlan::kTiles, 2, 256, 1};
+  if (M <= 32 && a_major == B200S_K_MAJOR && b_major == B200S_K_MAJOR) {
+    best.kind = LinearPlan::kSkinny;
+    return best;
+  }
+  // Estimated clocks of every tile shape and split: waves of tiles, each bound by the tensor cores (4096
+  // products a clock and SM) or by reading operands from L2 (60 bytes a clock and SM); partial products cost
+  // their traffic and a second launch.
+  const int64_t kb = (K + kBK - 1) / kBK;
+  double least = 0;
+  const struct { int cg, bn; } shapes[] = {{2, 256}, {2, 128}, {1, 128}};
+  for (const auto& s : shapes) {
+    const int64_t tiles = ((M + 128 * s.cg - 1) / (128 * s.cg)) * ((N + s.bn - 1) / s.bn);
+    const int64_t units = 148 / s.cg;
+    const double mma = s.bn / s.cg * s.cg * 0.5 * 4, fill = (128.0 + s.bn / s.cg) * kRowBytes / 60.0;
+    for (int split = 1; split <= 16 && split <= kb; ++split) {
+      const int64_t waves = (tiles * split + units - 1) / units;
+      const double tile = static_cast<double>((kb + split - 1) / split) * (mma > fill ? mma : fill) + 800;
+      double clocks = static_cast<double>(waves) * tile + 2500;
+      if (split > 1) clocks += 4500 + static_cast<double>(M) * static_cast<double>(N) * (8.0 * split + 2) / 4500;
+      if (least == 0 || clocks < least) {
+        least = clocks;
+        best.cta_group = s.cg, best.tile_n = s.bn, best.splits = split;
+      }
+    }
+  }
+  return best;
+}
+
+int launch_linear(const LinearArgs& g, const LinearPlan& plan, cudaStream_t stream) {
+  if (g.M > INT32_MAX || g.N > INT32_MAX || g.K > INT32_MAX) return B200S_ERR_BAD_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(g.A) & 15u) || (reinterpret_cast<uintptr_t>(g.B) & 15u)) return B200S_ERR_BAD_ALIGNMENT;
+  if ((g.lda * 2) % 16 || (g.ldb * 2) % 16) return B200S_ERR_BAD_STRIDE;
+  const bool bf16_out = g.out_dtype == B200S_BF16;
+  if (plan.kind == LinearPlan::kSkinny) {
+    const SkinnyParams p{static_cast<const uint16_t*>(g.A), static_cast<const uint16_t*>(g.B), g.bias, g.residual, g.C, g.preact,
+                         g.lda, g.ldb, g.ldc, g.ldr, g.ldz,
+                         static_cast<int32_t>(g.M), static_cast<int32_t>(g.N), static_cast<int32_t>(g.K), g.activation};
+    if (g.M <= 8) return launch_skinny<1>(p, bf16_out, stream);
+    if (g.M <= 16) return launch_skinny<2>(p, bf16_out, stream);
+    return launch_skinny<4>(p, bf16_out, stream);
+  }
+  const bool partial = plan.splits > 1;
+  uint32_t* status = device_status_words();
+  if (!status) return B200S_ERR_NO_DEVICE;
+  CUtensorMap maps[4];
+  const int cg = plan.cta_group, bn_cta = plan.tile_n / cg;
+  int rc = g.a_major == B200S_K_MAJOR ? encode_operand_map(&maps[0], g.A, g.in_dtype, g.M, g.K, g.lda, 1, 0, 128, false)
+                                      : encode_operand_map(&maps[0], g.A, g.in_dtype, g.K, g.M, g.lda, 1, 0, kBK, false);
+  if (rc) return rc;
+  rc = g.b_major == B200S_K_MAJOR ? encode_operand_map(&maps[1], g.B, g.in_dtype, g.N, g.K, g.ldb, 1, 0, bn_cta, false)
+                                  : encode_operand_map(&maps[1], g.B, g.in_dtype, g.K, g.N, g.ldb, 1, 0, kBK, false);
+  if (rc) return rc;
+  LinearParams p = {};
+  maps[2] = maps[3] = maps[0];     // never used unless built below
+  if (partial) {
+    rc = encode_operand_map(&maps[2], g.partials, B200S_FP32, g.M, g.N, g.ldp, plan.splits, g.M * g.ldp, 32, true);
+    if (rc) return rc;
+    p.tma_c = 1;
+  } else {
+    p.tma_c = tma_rows(g.C, g.ldc, g.M) && g.ldc >= g.N;
+    p.tma_z = g.preact && tma_rows(g.preact, g.ldz, g.M) && g.ldz >= g.N;
+    // (a single row needs no stride of its own, but the map wants a legal one)
+    const int64_t ldc = g.M > 1 ? g.ldc : (g.N + 7) / 8 * 8, ldz = g.M > 1 ? g.ldz : (g.N + 7) / 8 * 8;
+    if (p.tma_c && (rc = encode_operand_map(&maps[2], g.C, g.out_dtype, g.M, g.N, ldc, 1, 0, 32, true)) != 0) return rc;
+    if (p.tma_z && (rc = encode_operand_map(&maps[3], g.preact, g.out_dtype, g.M, g.N, ldz, 1, 0, 32, true)) != 0) return rc;
+  }
+  p.M = static_cast<int32_t>(g.M), p.N = static_cast<int32_t>(g.N), p.K = static_cast<int32_t>(g.K);
+  p.m_tiles = static_cast<int32_t>((g.M + 128 * cg - 1) / (128 * cg));
+  p.n_tiles = static_cast<int32_t>((g.N + plan.tile_n - 1) / plan.tile_n);
+  p.k_blocks = static_cast<int32_t>((g.K + kBK - 1) / kBK);
+  p.splits = plan.splits;
+  const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles * plan.splits;
+  if (total > INT32_MAX) return B200S_ERR_BAD_SHAPE;
+  p.total_tiles = static_cast<int32_t>(total);
+  p.raster_group = 8;
+  p.a_mn = g.a_major == B200S_MN_MAJOR, p.b_mn = g.b_major == B200S_MN_MAJOR;
+  p.fmt = g.in_dtype == B200S_BF16 ? 1 : 0;
+  p.bf16_out = bf16_out, p.act = g.activation;
+  p.bias = g.bias, p.residual = g.residual, p.C = g.C, p.Z = g.preact;
+  p.ldc = g.ldc, p.ldr = g.ldr, p.ldz = g.ldz;
+  p.vec_r = g.residual && tma_rows(g.residual, g.ldr, g.M) && g.N % 8 == 0;
+  p.status = status;
+  return partial ? launch_plan<true>(plan, maps, p, stream) : launch_plan<false>(plan, maps, p, stream);
+}
+
+}  // namespace b200s
