@@ -473,31 +473,40 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+template <bool BF16>
+__device__ __forceinline__ float from_bits(uint16_t u) {
+  if constexpr (BF16) return __uint_as_float(static_cast<uint32_t>(u) << 16);
+  return __half2float(__ushort_as_half(u));
+}
+template <bool BF16>
+__device__ __forceinline__ uint16_t to_bits(float v) {
+  if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  return __half_as_ushort(__float2half_rn(v));
+}
+
 struct SkinnyParams {
   const uint16_t* X;
   const uint16_t* W;
-  const void* bias;
-  const void* residual;
-  void* C;
-  void* Z;
+  const uint16_t* bias;       // where there is none: any readable element, with bias_step 0
+  const uint16_t* residual;   // the same, with res_step and ldr 0
+  uint16_t* C;
+  uint16_t* Z;
   int64_t ldx, ldw, ldc, ldr, ldz;
   int32_t M, N, K, act;
+  int32_t bias_step, res_step, has_z;
 };
 
 // 8 elements from column k of a row, zero from column K on (what lies there is not part of the operand).
+// Every load of this kernel is unconditional and its address in range by itself: beyond the row's last vector
+// the last one is read and dropped.
 __device__ __forceinline__ uint4 row8(const uint16_t* row, int k, int K, bool in) {
-  if (!in || k >= K) return make_uint4(0, 0, 0, 0);
-  uint4 q = __ldg(reinterpret_cast<const uint4*>(row + k));
-  if (k + 8 > K) {
-    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  const int last = (K - 1) & ~7;
+  uint4 q = __ldg(reinterpret_cast<const uint4*>(row + min(k, last)));
+  uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  const int left = in ? K - k : 0;       // elements of the vector that belong to the row
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (k + 2 * j >= K) w[j] = 0;
-      else if (k + 2 * j + 1 >= K) w[j] &= 0xffffu;
-    }
-    q = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  return q;
+  for (int j = 0; j < 4; ++j) w[j] = left >= 2 * j + 2 ? w[j] : (left == 2 * j + 1 ? w[j] & 0xffffu : 0u);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <int MT, bool BF16>
@@ -551,13 +560,13 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const SkinnyP
   __syncthreads();
   for (int i = threadIdx.x; i < 16 * 8 * MT; i += 32 * kSkinnyWarps) {
     const int n = i & 15, m = i >> 4;
-    if (m >= p.M || n0 + n >= p.N) continue;
+    const int row = min(m, p.M - 1), col = min(n0 + n, p.N - 1);
+    const float add = from_bits<BF16>(__ldg(p.bias + static_cast<int64_t>(col) * p.bias_step));
+    const float res = from_bits<BF16>(__ldg(p.residual + static_cast<int64_t>(row) * p.ldr + static_cast<int64_t>(col) * p.res_step));
     float z = 0.f;
 #pragma unroll
     for (int w = 0; w < kSkinnyWarps; ++w) z += part[w][n][m];
-    if (p.bias) z += element(p.bias, n0 + n, BF16);
-    using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-    if (p.Z) static_cast<T*>(p.Z)[static_cast<int64_t>(m) * p.ldz + n0 + n] = row::from_f<T>(z);
+    z += p.bias_step ? add : 0.f;
     float y = z;
     switch (p.act) {
       case B200S_ACT_RELU: y = epi::act_fast<B200S_ACT_RELU>(z); break;
@@ -567,8 +576,11 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const SkinnyP
       case B200S_ACT_GELU_TANH: y = epi::act_fast<B200S_ACT_GELU_TANH>(z); break;
       default: break;
     }
-    if (p.residual) y += row::to_f(static_cast<const T*>(p.residual)[static_cast<int64_t>(m) * p.ldr + n0 + n]);
-    static_cast<T*>(p.C)[static_cast<int64_t>(m) * p.ldc + n0 + n] = row::from_f<T>(y);
+    y += p.res_step ? res : 0.f;
+    if (m < p.M && n0 + n < p.N) {
+      if (p.has_z) p.Z[static_cast<int64_t>(m) * p.ldz + n0 + n] = to_bits<BF16>(z);
+      p.C[static_cast<int64_t>(m) * p.ldc + n0 + n] = to_bits<BF16>(y);
+    }
   }
 }
 
@@ -683,9 +695,13 @@ int launch_linear(const LinearArgs& g, const LinearPlan& plan, cudaStream_t stre
   if ((g.lda * 2) % 16 || (g.ldb * 2) % 16) return B200S_ERR_BAD_STRIDE;
   const bool bf16_out = g.out_dtype == B200S_BF16;
   if (plan.kind == LinearPlan::kSkinny) {
-    const SkinnyParams p{static_cast<const uint16_t*>(g.A), static_cast<const uint16_t*>(g.B), g.bias, g.residual, g.C, g.preact,
-                         g.lda, g.ldb, g.ldc, g.ldr, g.ldz,
-                         static_cast<int32_t>(g.M), static_cast<int32_t>(g.N), static_cast<int32_t>(g.K), g.activation};
+    SkinnyParams p = {};
+    p.X = static_cast<const uint16_t*>(g.A), p.W = static_cast<const uint16_t*>(g.B);
+    p.C = static_cast<uint16_t*>(g.C), p.Z = static_cast<uint16_t*>(g.preact), p.has_z = g.preact != nullptr;
+    p.bias = g.bias ? static_cast<const uint16_t*>(g.bias) : p.X, p.bias_step = g.bias ? 1 : 0;
+    p.residual = g.residual ? static_cast<const uint16_t*>(g.residual) : p.X, p.res_step = g.residual ? 1 : 0;
+    p.ldx = g.lda, p.ldw = g.ldb, p.ldc = g.ldc, p.ldr = g.residual ? g.ldr : 0, p.ldz = g.ldz;
+    p.M = static_cast<int32_t>(g.M), p.N = static_cast<int32_t>(g.N), p.K = static_cast<int32_t>(g.K), p.act = g.activation;
     if (g.M <= 8) return launch_skinny<1>(p, bf16_out, stream);
     if (g.M <= 16) return launch_skinny<2>(p, bf16_out, stream);
     return launch_skinny<4>(p, bf16_out, stream);

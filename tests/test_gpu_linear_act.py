@@ -127,6 +127,16 @@ def test_activations_and_types(b200s, act, dtype, m, k, n):
     run_case(b200s, x, w, None, r, act)
 
 
+@pytest.mark.parametrize("m", [1, 8, 16, 17, 32, 33])
+@pytest.mark.parametrize("bias,residual", [(False, False), (True, False), (False, True)])
+def test_few_rows_and_many_columns(b200s, m, bias, residual):
+    """Generated tokens against a wide layer, with and without bias and residual; 4096 columns of 1024 elements end where
+    their allocation does."""
+    x, w, b, r, dy = inputs(m, 1024, 4096, torch.bfloat16, bias, residual)
+    for act in ("none", "gelu"):
+        run_case(b200s, x, w, b, r, act, dy if m == 17 else None)
+
+
 @pytest.mark.parametrize("m", [1, 9, 40, 257])
 def test_strides_and_offsets(b200s, m):
     """x, weight, residual and the gradient as slices of wider tensors, off 16-byte boundaries and transposed."""
