@@ -417,6 +417,31 @@ int b200s_epilogue_backward(int64_t M, int64_t N, int dtype, int activation, con
                             void* workspace_device, size_t workspace_bytes, void* stream);
 
 /*
+ * The dense linear layer of 16-bit activations in one call each way: b200s_matmul_epilogue and its whole
+ * backward pass for x (M x K), weight (N x K), bias (N), residual and y (M x N), all of dtype
+ * (B200S_BF16 or B200S_FP16), rows contiguous:
+ *   y = act(x . weight^T + bias) + residual, z (the pre-activation) stored when given;
+ *   dz = dy * act'(z), dx = dz . weight, dweight = dz^T . x, dbias = column sums of dz.
+ * bias, residual, z may be NULL; so may dx, dweight and dbias, and z for B200S_ACT_NONE. Rows of any
+ * length, alignment and stride are accepted: operands TMA cannot address are copied to scratch first.
+ * M = 0 computes the gradients of an empty batch. Scratch, 256-byte aligned (NULL when the size is 0): the
+ * matching _workspace bytes, with copies = 0 when every operand (x, weight; for the backward pass dy too) starts
+ * on a 16-byte boundary and has rows a multiple of 16 bytes apart, else 1.
+ */
+int b200s_linear_act_workspace(int64_t M, int64_t N, int64_t K, int dtype, int copies, size_t* bytes_out);
+int b200s_linear_act(int64_t M, int64_t N, int64_t K, int dtype, int activation, const void* x_device, int64_t ldx,
+                     const void* weight_device, int64_t ldw, const void* bias_device, const void* residual_device,
+                     int64_t ldr, void* y_device, int64_t ldy, void* z_device, int64_t ldz, void* workspace_device,
+                     size_t workspace_bytes, void* stream);
+int b200s_linear_act_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, int activation, int copies,
+                                        size_t* bytes_out);
+int b200s_linear_act_backward(int64_t M, int64_t N, int64_t K, int dtype, int activation, const void* x_device,
+                              int64_t ldx, const void* weight_device, int64_t ldw, const void* z_device, int64_t ldz,
+                              const void* dy_device, int64_t lddy, void* dx_device, int64_t lddx,
+                              void* dweight_device, int64_t lddw, void* dbias_device, void* workspace_device,
+                              size_t workspace_bytes, void* stream);
+
+/*
  * Log probability of one given token per row of logits, the row's log-sum-exp, the entropy of its
  * distribution and its top_k (0..64) most likely tokens with their log probabilities; all outputs but
  * token ids are fp32. lse, entropy may be NULL; the top outputs hold top_k values per row, best first,

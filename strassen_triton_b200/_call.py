@@ -17,6 +17,16 @@ def dtype_code(t: torch.Tensor, what: str) -> int:
 
 def require_cuda(first: torch.Tensor, *others) -> None:
     """All of them (None aside) CUDA tensors of one device."""
+    try:
+        index = first.get_device()
+        if index >= 0:
+            for t in others:
+                if t is not None and t.get_device() != index:
+                    break
+            else:
+                return
+    except AttributeError:
+        pass
     for t in (first,) + others:
         if t is None:
             continue
@@ -55,6 +65,17 @@ def rows_of(t: torch.Tensor):
     if (m.stride(1) != 1 and d > 1) or m.stride(0) < 0:
         m = m.contiguous()
     return m, m.shape[0], m.stride(0)
+
+
+def once(backward):
+    """once_differentiable for an autograd function's backward, without its bookkeeping in the usual case that no
+    graph of the backward pass is being recorded."""
+    slow = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 def wants_grad(*tensors) -> bool:

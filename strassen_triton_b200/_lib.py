@@ -139,6 +139,12 @@ SIGNATURES = {
     "b200s_matmul_epilogue": (_INT, [_P(Problem), _P(Epilogue), _PTR, _PTR, _PTR, _PTR, _SIZE, _PTR]),
     "b200s_epilogue_backward_workspace": (_INT, [_I64, _I64, _P(_SIZE)]),
     "b200s_epilogue_backward": (_INT, [_I64, _I64, _INT, _INT, _PTR, _I64, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _SIZE, _PTR]),
+    "b200s_linear_act_workspace": (_INT, [_I64, _I64, _I64, _INT, _INT, _P(_SIZE)]),
+    "b200s_linear_act": (_INT, [_I64, _I64, _I64, _INT, _INT, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _I64, _PTR, _I64, _PTR, _I64,
+                                _PTR, _SIZE, _PTR]),
+    "b200s_linear_act_backward_workspace": (_INT, [_I64, _I64, _I64, _INT, _INT, _INT, _P(_SIZE)]),
+    "b200s_linear_act_backward": (_INT, [_I64, _I64, _I64, _INT, _INT, _PTR, _I64, _PTR, _I64, _PTR, _I64, _PTR, _I64, _PTR, _I64,
+                                         _PTR, _I64, _PTR, _PTR, _SIZE, _PTR]),
     "b200s_token_logprobs": (_INT, [_I64, _I64, _INT, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _INT, _PTR, _PTR, _PTR]),
     "b200s_token_logprobs_backward": (_INT, [_I64, _I64, _I64, _INT, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _PTR, _PTR,
                                              _I64, _PTR]),

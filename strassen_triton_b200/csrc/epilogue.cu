@@ -89,6 +89,28 @@ __global__ void __launch_bounds__(kThreads) epilogue_kernel(const EpiloguePass p
   }
 }
 
+// Rows copied to where TMA can address them (a padded leading dimension; the padding is left alone).
+template <int VEC>
+__global__ void __launch_bounds__(kThreads) pad_rows_kernel(const uint16_t* in, uint16_t* out, int64_t rows, int64_t cols, int64_t ld_in,
+                                                            int64_t ld_out) {
+  using P = Pack<uint16_t, VEC>;
+  constexpr int B = 4;
+  const int64_t per = cols / VEC, total = rows * per, step = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i0 < total; i0 += B * step) {
+    P v[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int64_t i = i0 + b * step;
+      if (i < total) v[b] = row::ld<P>(in + (i / per) * ld_in + (i % per) * VEC);
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int64_t i = i0 + b * step;
+      if (i < total) row::st(out + (i / per) * ld_out + (i % per) * VEC, v[b]);
+    }
+  }
+}
+
 struct EpilogueBwd {
   const void* z;
   const void* dy;
@@ -370,6 +392,173 @@ int b200s_epilogue_backward(int64_t M, int64_t N, int dtype, int activation, con
   column_sum_kernel<<<static_cast<unsigned>((N + 31) / 32), kSumThreads, 0, s>>>(part, dbias, N, slices, dtype);
   B200S_CUDA_OK(cudaGetLastError());
   count_launch();
+  return B200S_OK;
+}
+
+// ---- the dense 16-bit linear layer in one call each way ------------------------------------------
+
+static int64_t padded(int64_t n) { return (n + 7) / 8 * 8; }
+static size_t rows_bytes(int64_t rows, int64_t cols) { return round256(static_cast<size_t>(rows) * static_cast<size_t>(padded(cols)) * 2); }
+
+static size_t product_scratch(int64_t M, int64_t N, int64_t K, int a_major, int b_major) {
+  const LinearPlan plan = plan_linear(M, N, K, a_major, b_major);
+  return plan.splits > 1 ? round256(static_cast<size_t>(plan.splits) * static_cast<size_t>(M) * static_cast<size_t>(partial_ld(N)) * 4) : 0;
+}
+
+static int check_linear(int64_t M, int64_t N, int64_t K, int dtype, int activation) {
+  if (M < 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) return B200S_ERR_BAD_SHAPE;
+  if (dtype != B200S_BF16 && dtype != B200S_FP16) return B200S_ERR_BAD_DTYPE;
+  if (activation < B200S_ACT_NONE || activation > B200S_ACT_GELU_TANH) return B200S_ERR_BAD_ALGO;
+  return B200S_OK;
+}
+
+static bool addressable(const void* p, int64_t ld, int64_t rows, int64_t cols) {
+  return aligned(p, ld, rows, 2, 16) && (rows <= 1 || ld >= cols);
+}
+
+// `p`, or its rows copied to *scratch (which then moves on). *ld becomes the leading dimension to use.
+static int operand_rows(const void** p, int64_t* ld, int64_t rows, int64_t cols, uint8_t** scratch, cudaStream_t stream) {
+  if (addressable(*p, *ld, rows, cols)) {
+    if (rows <= 1) *ld = padded(cols);
+    return B200S_OK;
+  }
+  const uint16_t* in = static_cast<const uint16_t*>(*p);
+  uint16_t* out = reinterpret_cast<uint16_t*>(*scratch);
+  const int64_t to = padded(cols);
+  const bool pairs = cols % 2 == 0 && aligned(in, *ld, rows, 2, 4);
+  const int64_t blocks = (rows * cols / (pairs ? 2 : 1) + 4 * kThreads - 1) / (4 * kThreads);
+  const unsigned grid = static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16);
+  if (pairs)
+    pad_rows_kernel<2><<<grid, kThreads, 0, stream>>>(in, out, rows, cols, *ld, to);
+  else
+    pad_rows_kernel<1><<<grid, kThreads, 0, stream>>>(in, out, rows, cols, *ld, to);
+  B200S_CUDA_OK(cudaGetLastError());
+  count_launch();
+  *p = out;
+  *ld = to;
+  *scratch += rows_bytes(rows, cols);
+  return B200S_OK;
+}
+
+static int run_linear(LinearArgs g, uint8_t* scratch, cudaStream_t stream) {
+  const LinearPlan plan = plan_linear(g.M, g.N, g.K, g.a_major, g.b_major);
+  g.partials = reinterpret_cast<float*>(scratch);
+  g.ldp = partial_ld(g.N);
+  int rc = launch_linear(g, plan, stream);
+  if (rc || plan.splits == 1) return rc;
+  const EpiloguePass ep{g.partials, g.bias, g.residual, g.C, g.preact, g.M, g.N, g.ldp, g.ldr, g.ldc, g.ldz, plan.splits};
+  return run_pass(ep, g.out_dtype, g.activation, stream);
+}
+
+int b200s_linear_act_workspace(int64_t M, int64_t N, int64_t K, int dtype, int copies, size_t* bytes_out) {
+  if (!bytes_out) return B200S_ERR_NULL_POINTER;
+  int rc = check_linear(M, N, K, dtype, B200S_ACT_NONE);
+  if (rc) return rc;
+  *bytes_out = M == 0 ? 0 : product_scratch(M, N, K, B200S_K_MAJOR, B200S_K_MAJOR) + (copies ? rows_bytes(M, K) + rows_bytes(N, K) : 0);
+  return B200S_OK;
+}
+
+int b200s_linear_act(int64_t M, int64_t N, int64_t K, int dtype, int activation, const void* x, int64_t ldx,
+                     const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* y,
+                     int64_t ldy, void* z, int64_t ldz, void* workspace, size_t workspace_bytes, void* stream_v) {
+  int rc = check_linear(M, N, K, dtype, activation);
+  if (rc) return rc;
+  if (M == 0) return B200S_OK;
+  if (!x || !weight || !y) return B200S_ERR_NULL_POINTER;
+  if ((M > 1 && (ldx < 0 || (residual && ldr < 0) || ldy < N || (z && ldz < N))) || (N > 1 && ldw < 0)) return B200S_ERR_BAD_STRIDE;
+  for (const void* q : {x, weight, bias, residual, static_cast<const void*>(y), static_cast<const void*>(z)})
+    if (reinterpret_cast<uintptr_t>(q) & 1u) return B200S_ERR_BAD_ALIGNMENT;
+  size_t need = 0;
+  b200s_linear_act_workspace(M, N, K, dtype, !addressable(x, ldx, M, K) || !addressable(weight, ldw, N, K), &need);
+  if (need > 0) {
+    if (!workspace) return B200S_ERR_NULL_POINTER;
+    if (workspace_bytes < need) return B200S_ERR_WORKSPACE_TOO_SMALL;
+    if (reinterpret_cast<uintptr_t>(workspace) & 255u) return B200S_ERR_BAD_ALIGNMENT;
+  }
+  if (!device_status_words()) return B200S_ERR_NO_DEVICE;
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  uint8_t* scratch = static_cast<uint8_t*>(workspace);
+  if ((rc = operand_rows(&x, &ldx, M, K, &scratch, stream)) != 0) return rc;
+  if ((rc = operand_rows(&weight, &ldw, N, K, &scratch, stream)) != 0) return rc;
+  const LinearArgs g{x, weight, y, bias, residual, z, nullptr, M, N, K, ldx, ldw, ldy, ldr, ldz, 0, B200S_K_MAJOR, B200S_K_MAJOR, dtype, dtype, activation};
+  return run_linear(g, scratch, stream);
+}
+
+int b200s_linear_act_backward_workspace(int64_t M, int64_t N, int64_t K, int dtype, int activation, int copies, size_t* bytes_out) {
+  if (!bytes_out) return B200S_ERR_NULL_POINTER;
+  int rc = check_linear(M, N, K, dtype, activation);
+  if (rc) return rc;
+  size_t sums = 0;
+  b200s_epilogue_backward_workspace(M, N, &sums);
+  if (M == 0) {
+    *bytes_out = round256(sums);
+    return B200S_OK;
+  }
+  const size_t p1 = product_scratch(M, K, N, B200S_K_MAJOR, B200S_MN_MAJOR), p2 = product_scratch(N, K, M, B200S_MN_MAJOR, B200S_MN_MAJOR);
+  *bytes_out = (p1 > p2 ? p1 : p2) + round256(sums) + (copies || activation != B200S_ACT_NONE ? rows_bytes(M, N) : 0) +
+               (copies ? rows_bytes(M, K) + rows_bytes(N, K) : 0);
+  return B200S_OK;
+}
+
+int b200s_linear_act_backward(int64_t M, int64_t N, int64_t K, int dtype, int activation, const void* x, int64_t ldx,
+                              const void* weight, int64_t ldw, const void* z, int64_t ldz, const void* dy, int64_t lddy,
+                              void* dx, int64_t lddx, void* dweight, int64_t lddw, void* dbias, void* workspace,
+                              size_t workspace_bytes, void* stream_v) {
+  int rc = check_linear(M, N, K, dtype, activation);
+  if (rc) return rc;
+  if (!dx && !dweight && !dbias) return B200S_OK;
+  if (M > 0 && (!dy || (dweight && !x) || (dx && !weight) || (activation != B200S_ACT_NONE && !z))) return B200S_ERR_NULL_POINTER;
+  if ((M > 1 && (lddy < 0 || (dweight && ldx < 0) || (dx && lddx < K) || (activation != B200S_ACT_NONE && ldz < 0))) ||
+      (N > 1 && ((dx && ldw < 0) || (dweight && lddw < K))))
+    return B200S_ERR_BAD_STRIDE;
+  for (const void* q : {x, weight, z, dy, static_cast<const void*>(dx), static_cast<const void*>(dweight), static_cast<const void*>(dbias)})
+    if (reinterpret_cast<uintptr_t>(q) & 1u) return B200S_ERR_BAD_ALIGNMENT;
+  size_t need = 0;
+  const bool copies = M > 0 && (!addressable(dy, lddy, M, N) || (dweight && !addressable(x, ldx, M, K)) || (dx && !addressable(weight, ldw, N, K)));
+  b200s_linear_act_backward_workspace(M, N, K, dtype, activation, copies, &need);
+  if (!workspace) return B200S_ERR_NULL_POINTER;
+  if (workspace_bytes < need) return B200S_ERR_WORKSPACE_TOO_SMALL;
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return B200S_ERR_BAD_ALIGNMENT;
+  if (!device_status_words()) return B200S_ERR_NO_DEVICE;
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  uint8_t* scratch = static_cast<uint8_t*>(workspace);
+  size_t sums = 0;
+  b200s_epilogue_backward_workspace(M, N, &sums);
+  void* parts = scratch;
+  scratch += round256(sums);
+  if (M == 0) {
+    if (dweight)
+      B200S_CUDA_OK(cudaMemset2DAsync(dweight, static_cast<size_t>(N > 1 ? lddw : K) * 2, 0, static_cast<size_t>(K) * 2, static_cast<size_t>(N), stream));
+    if (dbias) B200S_CUDA_OK(cudaMemsetAsync(dbias, 0, static_cast<size_t>(N) * 2, stream));
+    return B200S_OK;
+  }
+  // dz: dy itself where nothing has to be multiplied into it and TMA can read it
+  const bool products = dx || dweight;
+  const bool own = products && (activation != B200S_ACT_NONE || !addressable(dy, lddy, M, N));
+  const void* dz = dy;
+  int64_t lddz = M > 1 ? lddy : padded(N);
+  if (own) {
+    dz = scratch, lddz = padded(N);
+    scratch += rows_bytes(M, N);
+  }
+  if (own || dbias) {
+    rc = b200s_epilogue_backward(M, N, dtype, activation, z, ldz, dy, lddy, own ? const_cast<void*>(dz) : nullptr, lddz, dbias, parts, sums, stream_v);
+    if (rc) return rc;
+  }
+  if (dx) {
+    if ((rc = operand_rows(&weight, &ldw, N, K, &scratch, stream)) != 0) return rc;
+  }
+  if (dweight) {
+    if ((rc = operand_rows(&x, &ldx, M, K, &scratch, stream)) != 0) return rc;
+  }
+  if (dx) {
+    const LinearArgs g{dz, weight, dx, nullptr, nullptr, nullptr, nullptr, M, K, N, lddz, ldw, lddx, 0, 0, 0, B200S_K_MAJOR, B200S_MN_MAJOR, dtype, dtype, B200S_ACT_NONE};
+    if ((rc = run_linear(g, scratch, stream)) != 0) return rc;
+  }
+  if (dweight) {
+    const LinearArgs g{dz, x, dweight, nullptr, nullptr, nullptr, nullptr, N, K, M, lddz, ldx, lddw, 0, 0, 0, B200S_MN_MAJOR, B200S_MN_MAJOR, dtype, dtype, B200S_ACT_NONE};
+    if ((rc = run_linear(g, scratch, stream)) != 0) return rc;
+  }
   return B200S_OK;
 }
 

@@ -14,7 +14,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._call import call, dtype_code, ptr, require_cuda, rows_of, wants_grad
+from ._call import call, dtype_code, once, ptr, require_cuda, rows_of, wants_grad
 
 
 class TokenLogprobs(NamedTuple):
@@ -41,8 +41,8 @@ def _forward(logits, targets, vocab, ignore_index, entropy, top_k, lse):
 def _backward(logits, targets, vocab, ignore_index, lse, entropy, dlogprob, dentropy):
     xr, rows, ld = rows_of(logits)
     t = targets.contiguous()
-    dl = dlogprob.to(torch.float32).contiguous() if dlogprob is not None else None
-    de = dentropy.to(torch.float32).contiguous() if dentropy is not None else None
+    dl, de = (g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.to(torch.float32).contiguous()
+              for g in (dlogprob, dentropy))
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     width = logits.shape[-1]
     call(logits.device, _lib.load().b200s_token_logprobs_backward, rows, vocab, width, dtype_code(logits, "logits"),
@@ -63,7 +63,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
         return lp, ent, ids, top
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dlp, dent, _dids, _dtop):
         logits, targets, lse, ent = ctx.saved_tensors
         if dlp is None and dent is None:

@@ -8,6 +8,7 @@ and the bias's gradient over the rows has a fixed order: the same call gives the
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -15,7 +16,7 @@ import torch.nn as nn
 from torch import Tensor
 
 from . import _lib
-from ._call import call, dtype_code, ptr, require_cuda, rows_of, wants_grad
+from ._call import DTYPE, call, dtype_code, once, ptr, require_cuda, rows_of, wants_grad
 
 
 def _check(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]) -> None:
@@ -35,90 +36,97 @@ def _check(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]) -> None:
         raise TypeError(f"weight and bias must be of one type, got {weight.dtype} and {bias.dtype}")
 
 
-def _param_code(x, weight, bias):
-    p = weight if weight is not None else bias
-    return dtype_code(p if p is not None else x, "weight")
+def _dense(p):
+    return p if p is None or p.is_contiguous() else p.contiguous()
 
 
 def _forward(x, weight, bias, eps, stats):
-    """(y, mean, rstd); the statistics are None unless ``stats``."""
+    """(y, statistics): two rows of fp32 values, mean and rstd, or None without ``stats``."""
     xr, rows, ldx = rows_of(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if stats:
-        mean = torch.empty(rows, dtype=torch.float32, device=x.device)
-        rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
-    w = weight.contiguous() if weight is not None else None
-    b = bias.contiguous() if bias is not None else None
+    y = torch.empty_like(x) if xr is x and x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    w, b = _dense(weight), _dense(bias)
     d = x.shape[-1]
-    call(x.device, _lib.load().b200s_layer_norm, rows, d, dtype_code(x, "x"), _param_code(x, w, b), eps, xr.data_ptr(), ldx,
-         ptr(w), ptr(b), y.data_ptr(), d, ptr(mean), ptr(rstd))
-    return y, mean, rstd
+    p = w if w is not None else b
+    st, mean, rstd = None, None, None
+    if stats:
+        st = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        mean = st.data_ptr()
+        rstd = mean + 4 * rows
+        if rows == 0:
+            mean = rstd = None
+    code = DTYPE[x.dtype]
+    call(x.device, _lib.load().b200s_layer_norm, rows, d, code, code if p is None else DTYPE[p.dtype], eps, xr.data_ptr(), ldx,
+         ptr(w), ptr(b), y.data_ptr(), d, mean, rstd)
+    return y, st
 
 
-def _backward(dy, x, weight, mean, rstd, param_dtype, need_x, need_w, need_b):
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(rows, d):
+    n = ctypes.c_size_t(0)
+    _lib.check(_lib.load().b200s_layer_norm_backward_workspace(rows, d, ctypes.byref(n)))
+    return n.value
+
+
+def _backward(dy, x, weight, st, param_dtype, need_x, need_w, need_b):
     """(dx, dw, db), None where not needed."""
-    lib = _lib.load()
     if dy.dtype != x.dtype:
         dy = dy.to(x.dtype)
     xr, rows, ldx = rows_of(x)
     gr, _, ldg = rows_of(dy)
-    d = x.shape[-1]
-    w = weight.contiguous() if weight is not None else None
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-    dw = torch.empty(d, dtype=param_dtype, device=x.device) if need_w else None
-    db = torch.empty(d, dtype=param_dtype, device=x.device) if need_b else None
+    d, dev = x.shape[-1], x.device
+    w = _dense(weight)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    dw = torch.empty(d, dtype=param_dtype, device=dev) if need_w else None
+    db = torch.empty(d, dtype=param_dtype, device=dev) if need_b else None
     ws, need = None, 0
     if need_w or need_b:
-        n = ctypes.c_size_t(0)
-        _lib.check(lib.b200s_layer_norm_backward_workspace(rows, d, ctypes.byref(n)))
-        need = n.value
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-    pd = _lib.FP32 if param_dtype == torch.float32 else dtype_code(x, "x")
-    call(x.device, lib.b200s_layer_norm_backward, rows, d, dtype_code(x, "x"), pd, xr.data_ptr(), ldx, gr.data_ptr(), ldg,
-         ptr(w), mean.data_ptr(), rstd.data_ptr(), ptr(dx), d, ptr(dw), ptr(db), ptr(ws), need)
+        need = _workspace_bytes(rows, d)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr()     # freed and reused in stream order
+    mean = st.data_ptr()
+    call(dev, _lib.load().b200s_layer_norm_backward, rows, d, DTYPE[x.dtype], DTYPE[param_dtype], xr.data_ptr(), ldx,
+         gr.data_ptr(), ldg, ptr(w), mean, mean + 4 * rows, ptr(dx), d, ptr(dw), ptr(db), ws, need)
     return dx, dw, db
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, st = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, st)
         p = weight if weight is not None else bias
         ctx.param_dtype = x.dtype if p is None else p.dtype
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight, st = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dw, db = _backward(dy, x, weight, mean, rstd, ctx.param_dtype, need[0], need[1], need[2])
+        dx, dw, db = _backward(dy, x, weight, st, ctx.param_dtype, need[0], need[1], need[2])
         return dx, dw, db, None
 
 
 # Opaque operators for traced graphs (torch.compile), as for the product (ops.py).
 @torch.library.custom_op("b200s::layer_norm", mutates_args=())
 def _layer_norm_op(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor],
-                   eps: float) -> tuple[Tensor, Tensor, Tensor]:
+                   eps: float) -> tuple[Tensor, Tensor]:
     return _forward(x, weight, bias, eps, True)
 
 
 @_layer_norm_op.register_fake
 def _(x, weight, bias, eps):
     rows = x.numel() // x.shape[-1]
-    return x.new_empty(x.shape), x.new_empty((rows,), dtype=torch.float32), x.new_empty((rows,), dtype=torch.float32)
+    return x.new_empty(x.shape), x.new_empty((2, rows), dtype=torch.float32)
 
 
 @torch.library.custom_op("b200s::layer_norm_backward", mutates_args=())
-def _layer_norm_backward_op(dy: Tensor, x: Tensor, weight: Optional[Tensor], mean: Tensor, rstd: Tensor,
+def _layer_norm_backward_op(dy: Tensor, x: Tensor, weight: Optional[Tensor], st: Tensor,
                             fp32_params: bool) -> tuple[Tensor, Tensor, Tensor]:
-    return _backward(dy, x, weight, mean, rstd, torch.float32 if fp32_params else x.dtype, True, True, True)
+    return _backward(dy, x, weight, st, torch.float32 if fp32_params else x.dtype, True, True, True)
 
 
 @_layer_norm_backward_op.register_fake
-def _(dy, x, weight, mean, rstd, fp32_params):
+def _(dy, x, weight, st, fp32_params):
     pd = torch.float32 if fp32_params else x.dtype
     d = x.shape[-1]
     return x.new_empty(x.shape), x.new_empty((d,), dtype=pd), x.new_empty((d,), dtype=pd)
@@ -126,16 +134,15 @@ def _(dy, x, weight, mean, rstd, fp32_params):
 
 def _op_setup(ctx, inputs, output):
     x, weight, bias, _ = inputs
-    _, mean, rstd = output
-    ctx.save_for_backward(x, weight, mean, rstd)
+    ctx.save_for_backward(x, weight, output[1])
     p = weight if weight is not None else bias
     ctx.fp32_params = p is not None and p.dtype == torch.float32
     ctx.has_bias = bias is not None
 
 
-def _op_backward(ctx, dy, _dmean, _drstd):
-    x, weight, mean, rstd = ctx.saved_tensors
-    dx, dw, db = _layer_norm_backward_op(dy, x, weight, mean, rstd, ctx.fp32_params)
+def _op_backward(ctx, dy, _dst):
+    x, weight, st = ctx.saved_tensors
+    dx, dw, db = _layer_norm_backward_op(dy, x, weight, st, ctx.fp32_params)
     return dx, dw if weight is not None else None, db if ctx.has_bias else None, None
 
 

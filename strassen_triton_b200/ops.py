@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -405,6 +406,90 @@ def _linear_act_backward(dy, x, weight, z, act, algo, depth, precision, need_x, 
     return dx, dw, db
 
 
+# The dense layer of 16-bit operands with contiguous rows: one call of the library each way.
+@functools.lru_cache(maxsize=1024)
+def _dense_workspace(backward, M, N, K, code, act, copies):
+    n = ctypes.c_size_t(0)
+    lib = _lib.load()
+    if backward:
+        _lib.check(lib.b200s_linear_act_backward_workspace(M, N, K, code, act, copies, ctypes.byref(n)))
+    else:
+        _lib.check(lib.b200s_linear_act_workspace(M, N, K, code, copies, ctypes.byref(n)))
+    return n.value
+
+
+def _off_grid(t) -> bool:
+    """Does TMA need a copy of these rows?"""
+    return t.data_ptr() % 16 != 0 or t.stride(0) % 8 != 0 or t.stride(0) < t.shape[1]
+
+
+def _rows_contiguous(t) -> bool:
+    return (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= 0
+
+
+def _dense_forward(x, weight, bias, residual, act, save):
+    """(y, z): z has its rows padded to whole 16-byte vectors, None when the backward pass needs none."""
+    M, K = x.shape
+    N, dt, dev = weight.shape[0], x.dtype, x.device
+    y = torch.empty((M, N), dtype=dt, device=dev)
+    z, ldz = None, 0
+    if save and act:
+        ldz = (N + 7) // 8 * 8
+        z = torch.empty((M, ldz), dtype=dt, device=dev)
+    rp, ldr = None, 0
+    if residual is not None:
+        if not _rows_contiguous(residual):
+            residual = residual.contiguous()
+        rp, ldr = residual.data_ptr(), residual.stride(0)
+    code = _DTYPE[dt]
+    need = _dense_workspace(False, M, N, K, code, 0, 1 if _off_grid(x) or _off_grid(weight) else 0)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr() if need else None     # reused in stream order
+    _call.call(dev, _lib.load().b200s_linear_act, M, N, K, code, act, x.data_ptr(), x.stride(0), weight.data_ptr(),
+               weight.stride(0), None if bias is None else bias.data_ptr(), rp, ldr, y.data_ptr(), N,
+               None if z is None else z.data_ptr(), ldz, ws, need)
+    return y, z
+
+
+def _dense_backward(dy, x, weight, z, act, need_x, need_w, need_b):
+    M, K = x.shape
+    N, dt, dev = weight.shape[0], x.dtype, x.device
+    if dy.dtype != dt:
+        dy = dy.to(dt)
+    if not _rows_contiguous(dy):
+        dy = dy.contiguous()
+    dx = torch.empty((M, K), dtype=dt, device=dev) if need_x else None
+    dw = torch.empty((N, K), dtype=dt, device=dev) if need_w else None
+    db = torch.empty(N, dtype=dt, device=dev) if need_b else None
+    code = _DTYPE[dt]
+    need = _dense_workspace(True, M, N, K, code, act, 1 if _off_grid(x) or _off_grid(weight) or _off_grid(dy) else 0)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr()
+    p = _call.ptr
+    _call.call(dev, _lib.load().b200s_linear_act_backward, M, N, K, code, act, x.data_ptr(), x.stride(0), weight.data_ptr(),
+               weight.stride(0), p(z), z.shape[1] if z is not None else 0, dy.data_ptr(), dy.stride(0), p(dx), K, p(dw), K,
+               p(db), ws, need)
+    return dx, dw, db
+
+
+class _DenseLinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        need = ctx.needs_input_grad
+        y, z = _dense_forward(x, weight, bias, residual, act, need[0] or need[1] or need[2])
+        ctx.save_for_backward(x, weight, z)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @_call.once
+    def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if need[0] or need[1] or need[2]:
+            x, weight, z = ctx.saved_tensors
+            dx, dw, db = _dense_backward(dy, x, weight, z, ctx.act, need[0], need[1], need[2])
+        return dx, dw, db, dy if need[3] else None, None
+
+
 class _LinearActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, algo, depth, precision):
@@ -415,7 +500,7 @@ class _LinearActFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_call.once
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -491,7 +576,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     if bias is not None:
         if bias.shape != out_shape[-1:]:
             raise ValueError(f"bias must hold {out_shape[-1]} elements, got shape {tuple(bias.shape)}")
-        bias = bias.to(x.dtype).contiguous()
+        if bias.dtype != x.dtype or not bias.is_contiguous():
+            bias = bias.to(x.dtype).contiguous()
     if residual is not None:
         if residual.shape != out_shape:
             raise ValueError(f"residual must have the shape of the result {tuple(out_shape)}, got {tuple(residual.shape)}")
@@ -501,7 +587,13 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
             residual = residual.reshape(-1, out_shape[-1])
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     depth = int(depth)
-    if torch.compiler.is_compiling():
+    if (algo == "dense" and x.dtype != torch.float32 and _rows_contiguous(x2) and _rows_contiguous(weight)
+            and not torch.compiler.is_compiling()):
+        if _call.wants_grad(x, weight, bias, residual):
+            y = _DenseLinearFn.apply(x2, weight, bias, residual, act)
+        else:
+            y = _dense_forward(x2, weight, bias, residual, act, False)[0]
+    elif torch.compiler.is_compiling():
         y = _linear_act_op(x2, weight, bias, residual, act, algo, depth, precision or "")[0]
     elif _call.wants_grad(x, weight, bias, residual):
         y = _LinearActFn.apply(x2, weight, bias, residual, act, algo, depth, precision)

@@ -85,6 +85,38 @@ def test_epilogue_arguments(lib):
     assert back(N=0) == _lib.ERR_BAD_SHAPE and back(dt=3) == _lib.ERR_BAD_DTYPE and back(dy=17) == _lib.ERR_BAD_ALIGNMENT
 
 
+def test_linear_arguments(lib):
+    n = ctypes.c_size_t(0)
+    size = ctypes.byref(n)
+    assert lib.b200s_linear_act_workspace(4, 8, 8, _lib.FP32, 0, size) == _lib.ERR_BAD_DTYPE
+    assert lib.b200s_linear_act_workspace(4, 0, 8, _lib.BF16, 0, size) == _lib.ERR_BAD_SHAPE
+    assert lib.b200s_linear_act_workspace(4, 8, 8, _lib.BF16, 0, None) == _lib.ERR_NULL_POINTER
+    assert lib.b200s_linear_act_workspace(4, 8, 8, _lib.BF16, 0, size) == 0 and n.value == 0
+    assert lib.b200s_linear_act_workspace(4, 8, 7, _lib.BF16, 1, size) == 0 and n.value >= (4 + 8) * 8 * 2
+    f = lib.b200s_linear_act
+    args = dict(M=4, N=8, K=8, dt=_lib.BF16, act=_lib.ACT_GELU, x=16, ldx=8, w=16, ldw=8, b=16, r=16, ldr=8, y=16, ldy=8, z=16,
+                ldz=8, ws=None, n=0)
+
+    def call(**kw):
+        return f(*{**args, **kw}.values(), None)
+
+    assert call(x=None) == _lib.ERR_NULL_POINTER and call(act=7) == _lib.ERR_BAD_ALGO and call(ldy=7) == _lib.ERR_BAD_STRIDE
+    assert call(ldz=7) == _lib.ERR_BAD_STRIDE and call(ldx=-8) == _lib.ERR_BAD_STRIDE and call(r=17) == _lib.ERR_BAD_ALIGNMENT
+    assert call(x=18) == _lib.ERR_NULL_POINTER                     # a copy of x needs scratch
+    assert call(x=18, ws=256, n=16) == _lib.ERR_WORKSPACE_TOO_SMALL and call(x=18, ws=128, n=1 << 20) == _lib.ERR_BAD_ALIGNMENT
+    assert call(M=0, x=None, y=None) == 0
+    g = lib.b200s_linear_act_backward
+    args2 = dict(M=4, N=8, K=8, dt=_lib.BF16, act=_lib.ACT_GELU, x=16, ldx=8, w=16, ldw=8, z=16, ldz=8, dy=16, ldy=8, dx=16, lddx=8,
+                 dw=16, lddw=8, db=16, ws=256, n=1 << 20)
+
+    def back(**kw):
+        return g(*{**args2, **kw}.values(), None)
+
+    assert back(z=None) == _lib.ERR_NULL_POINTER and back(dy=None) == _lib.ERR_NULL_POINTER and back(ws=None) == _lib.ERR_NULL_POINTER
+    assert back(n=8) == _lib.ERR_WORKSPACE_TOO_SMALL and back(lddx=7) == _lib.ERR_BAD_STRIDE and back(dw=17) == _lib.ERR_BAD_ALIGNMENT
+    assert back(dx=None, dw=None, db=None) == 0
+
+
 def test_logprob_arguments(lib):
     f = lib.b200s_token_logprobs
     args = dict(rows=4, vocab=8, dt=_lib.BF16, x=16, ld=8, t=16, ig=-100, lp=16, lse=16, ent=16, k=2, ids=16, top=16)
