@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include "../../include/b200s.h"
+#include "rowwise_device.cuh"
 
 namespace b200s {
 namespace epi {
@@ -85,6 +86,38 @@ __device__ __forceinline__ float act_fast(float z) {
   if constexpr (ACT == B200S_ACT_GELU_TANH) return z * fast_sigmoid(2.f * kTanhC * fmaf(kTanhA * z, z * z, z));
   return act<ACT>(z);
 }
+// Two values at a time, with the packed fp32 instructions (the same arithmetic as act_fast).
+__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
+template <int ACT>
+__device__ __forceinline__ float2 act_fast2(float2 z) {
+  using row::add_;
+  using row::fma_;
+  using row::mul_;
+  if constexpr (ACT == B200S_ACT_SILU || ACT == B200S_ACT_GELU_TANH) {
+    float2 u;
+    if constexpr (ACT == B200S_ACT_SILU)
+      u = mul_(z, pair(-2.f * kHalfLog2e));
+    else
+      u = mul_(mul_(z, pair(-4.f * kHalfLog2e * kTanhC)), fma_(mul_(z, z), pair(kTanhA), pair(1.f)));
+    const float2 d = add_(make_float2(ex2(u.x), ex2(u.y)), pair(1.f));
+    return mul_(z, make_float2(rcp(d.x), rcp(d.y)));
+  } else if constexpr (ACT == B200S_ACT_GELU) {
+    const float2 a = make_float2(fminf(fabsf(z.x), 30.f), fminf(fabsf(z.y), 30.f));
+    const float2 h = mul_(mul_(a, a), pair(-kHalfLog2e));
+    const float2 d = fma_(a, pair(0.35f), pair(1.f));
+    const float2 t = make_float2(rcp(d.x), rcp(d.y));
+    float2 q = fma_(t, pair(0.10458728923f), pair(-0.29827082271f));      // -P(t)
+    q = fma_(q, t, pair(0.00994253091f));
+    q = fma_(q, t, pair(-0.18356833940f));
+    q = fma_(q, t, pair(-0.13218160375f));
+    q = fma_(q, t, pair(-0.00050789281f));
+    q = mul_(q, make_float2(ex2(h.x), ex2(h.y)));
+    return fma_(a, q, make_float2(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y));
+  } else {
+    return make_float2(act<ACT>(z.x), act<ACT>(z.y));
+  }
+}
+
 template <int ACT>
 __device__ __forceinline__ float dact_fast(float z) {
   if constexpr (ACT == B200S_ACT_SILU) {

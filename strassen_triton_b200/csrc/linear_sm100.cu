@@ -3,9 +3,9 @@
 //
 // Two kernels:
 //   linear_kernel   tcgen05 tiles. Warp 0 loads 128-byte-swizzled operand tiles by TMA, one lane of warp 1
-//                   issues tcgen05.mma into one of two accumulators in tensor memory, warps 2..9 take the
+//                   issues tcgen05.mma into one of two accumulators in tensor memory, warps 2.. take the
 //                   other one through the epilogue: bias, activation, residual, staging in shared memory,
-//                   TMA stores. Tile shapes 256 x 256 and 256 x 128 (CTA pairs), 128 x 128; K may be cut into
+//                   TMA stores. Tile shapes 256 x 256 and 256 x 128 (CTA pairs), 128 x 128, 128 x 64; K may be cut into
 //                   parts whose fp32 partial products a second pass adds up (plan_linear weighs all this).
 //   skinny_kernel   up to 32 rows of A (tokens being generated) against K-major weights: bound by reading the
 //                   weights once, with mma.sync fed straight from global memory in registers.
@@ -31,8 +31,9 @@ namespace {
 
 constexpr int kRowBytes = 128;   // one swizzled row of a tile: 64 elements
 constexpr int kBK = 64;          // K elements per stage
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
+// Epilogue warps: four for every 64 columns of a tile, eight at most.
+template <int BN>
+constexpr int epi_warps = BN >= 128 ? 8 : 4;
 
 // Role codes in the status words when a wait runs out.
 enum : uint32_t { kWhoProducer = 13, kWhoMma = 14, kWhoMmaAcc = 15, kWhoEpilogue = 16 };
@@ -86,11 +87,11 @@ __device__ __forceinline__ float element(const void* p, int64_t i, bool bf16) {
 }
 
 template <int ACT>
-__device__ __forceinline__ void activate(float (&v)[64]) {
+__device__ __forceinline__ void activate(float2 (&v)[32]) {
 #pragma unroll
-  for (int j = 0; j < 64; ++j) v[j] = epi::act_fast<ACT>(v[j]);
+  for (int j = 0; j < 32; ++j) v[j] = epi::act_fast2<ACT>(v[j]);
 }
-__device__ __forceinline__ void activate(float (&v)[64], int act) {
+__device__ __forceinline__ void activate(float2 (&v)[32], int act) {
   switch (act) {      // the same for the whole launch
     case B200S_ACT_RELU: activate<B200S_ACT_RELU>(v); break;
     case B200S_ACT_RELU2: activate<B200S_ACT_RELU2>(v); break;
@@ -133,9 +134,10 @@ __device__ __forceinline__ void store_block(const CUtensorMap* map, bool tma, vo
 }
 
 template <int CG, int BN, int STAGES, bool PARTIAL>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(64 + 32 * epi_warps<BN>, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
               const __grid_constant__ CUtensorMap tmZ, const LinearParams p) {
+  constexpr int kEpiWarps = epi_warps<BN>;
   constexpr int BN_CTA = BN / CG;
   constexpr int A_BYTES = 128 * kRowBytes;
   constexpr int B_BYTES = BN_CTA * kRowBytes;
@@ -281,7 +283,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     // ------------------------------------------------------------ epilogue
     const int ew = warp - 2;
     const int lane_group = warp & 3;        // this warp's TMEM lanes [32 * lane_group, +32)
-    const int half = ew >> 2;               // and half of the tile's columns
+    const int half = ew >> 2;               // and share of the tile's columns
+    constexpr int WN = BN / (kEpiWarps / 4);
     const uint32_t stg = staging + static_cast<uint32_t>(ew) * 8192u;
     const bool bf16 = p.bf16_out != 0;
     int flip = 0, it = 0;
@@ -300,8 +303,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       const Tile t = decode(p, tile);
       const int buf = it & 1;
       const int row0 = t.mt * (128 * CG) + static_cast<int>(rank) * 128 + lane_group * 32;
-      const int col_first = t.nt * BN + half * (BN / 2);
-      constexpr int GROUPS = BN / 2 / 64;
+      const int col_first = t.nt * BN + half * WN;
+      constexpr int GROUPS = WN / 64;
       // residual of the first columns: on its way while the product is computed (a row of 64 columns is 8 lanes)
       uint4 res[8];
       auto fetch_residual = [&](int col0) {
@@ -315,12 +318,24 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       };
       const bool vec_res = !PARTIAL && p.residual != nullptr && p.vec_r;
       if (vec_res) fetch_residual(col_first);
+      // so is the bias: two columns of it per lane and group, handed round with the sums
+      uint32_t bias2[GROUPS];
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        bias2[g] = 0;
+        const int c = col_first + g * 64 + 2 * lane;
+        if (!PARTIAL && p.bias != nullptr) {
+          const uint16_t* bp = static_cast<const uint16_t*>(p.bias);
+          const uint32_t lo = c < p.N ? __ldg(bp + c) : 0, hi = c + 1 < p.N ? __ldg(bp + c + 1) : 0;
+          bias2[g] = lo | hi << 16;
+        }
+      }
       int ok = 1;
       if (lane == 0) ok = ptx::mbar_wait<CG == 2, 32>(tfull_bar(buf), (it >> 1) & 1u, abort_word, kWhoEpilogue) ? 1 : 0;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       ptx::tc_fence_after_sync();
-      const uint32_t taddr = tmem + (static_cast<uint32_t>(lane_group * 32) << 16) + static_cast<uint32_t>(buf * BN + half * (BN / 2));
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(lane_group * 32) << 16) + static_cast<uint32_t>(buf * BN + half * WN);
 #pragma unroll 1
       for (int g = 0; g < GROUPS; ++g) {
         const int col0 = col_first + g * 64;
@@ -355,33 +370,23 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
             sent();
           }
         } else {
-          float v[64];
+          float2 v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r0[j]), v[32 + j] = __uint_as_float(r1[j]);
+          for (int j = 0; j < 16; ++j) {
+            v[j] = make_float2(__uint_as_float(r0[2 * j]), __uint_as_float(r0[2 * j + 1]));
+            v[16 + j] = make_float2(__uint_as_float(r1[2 * j]), __uint_as_float(r1[2 * j + 1]));
+          }
           if (p.bias != nullptr) {
-            if (col0 + 64 <= p.N && ((reinterpret_cast<uintptr_t>(p.bias) + 2u * static_cast<uintptr_t>(col0)) & 15u) == 0) {
-              const uint4* bp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.bias) + col0);
+            uint32_t mine = bias2[0];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const uint4 q = __ldg(bp + j);
-                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+            for (int k = 1; k < GROUPS; ++k) mine = g == k ? bias2[k] : mine;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const float2 f = unpack2(w[k], bf16);
-                  v[8 * j + 2 * k] += f.x;
-                  v[8 * j + 2 * k + 1] += f.y;
-                }
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 64; ++j)
-                if (col0 + j < p.N) v[j] += element(p.bias, col0 + j, bf16);
-            }
+            for (int j = 0; j < 32; ++j) v[j] = row::add_(v[j], unpack2(__shfl_sync(0xffffffffu, mine, j), bf16));
           }
           uint32_t h[32];
           if (p.Z != nullptr) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) h[j] = pack2(v[2 * j], v[2 * j + 1], bf16);
+            for (int j = 0; j < 32; ++j) h[j] = pack2(v[j].x, v[j].y, bf16);
             store_block(&tmZ, p.tma_z != 0, p.Z, p.ldz, p.M, p.N, row0, col0, next_buffer(), h, lane);
             sent();
           }
@@ -417,16 +422,12 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
               const uint4 q = ptx::ld_shared_v4(b + static_cast<uint32_t>(lane) * 128u + ((static_cast<uint32_t>(j) ^ static_cast<uint32_t>(lane & 7)) << 4));
               const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 f = unpack2(w[k], bf16);
-                v[8 * j + 2 * k] += f.x;
-                v[8 * j + 2 * k + 1] += f.y;
-              }
+              for (int k = 0; k < 4; ++k) v[4 * j + k] = row::add_(v[4 * j + k], unpack2(w[k], bf16));
             }
             __syncwarp();
           }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) h[j] = pack2(v[2 * j], v[2 * j + 1], bf16);
+          for (int j = 0; j < 32; ++j) h[j] = pack2(v[j].x, v[j].y, bf16);
           store_block(&tmC, p.tma_c != 0, p.C, p.ldc, p.M, p.N, row0, col0, b, h, lane);
           sent();
         }
@@ -457,8 +458,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
 // y^T = W x^T with mma.sync m16n8k16: 16 rows of W (outputs) are the A operand, up to 8 * MT rows of x the
 // columns of B. The order of the terms along K is free as long as both operands agree, so lane (g, t) of a
 // warp takes 8 consecutive k of its rows, one 16-byte load, as the fragments of two steps: chunks of 32 k are
-// read whole, 64 bytes a row, without shared memory. The block's 8 warps take every 8th chunk and add up
-// their 16 x 8 MT sums in shared memory.
+// read whole, 64 bytes a row, without shared memory. The block's 8 warps take turns over runs of UN chunks and
+// add up their sums, 16 NT x 8 MT each, in shared memory.
 constexpr int kSkinnyWarps = 8;
 
 template <bool BF16>
@@ -509,63 +510,74 @@ __device__ __forceinline__ uint4 row8(const uint16_t* row, int k, int K, bool in
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int MT, bool BF16>
+template <int MT, int NT, bool BF16>
 __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const SkinnyParams p) {
-  constexpr int UN = MT <= 2 ? 4 : 2;       // chunks on their way per warp
-  __shared__ float part[kSkinnyWarps][16][8 * MT + 1];
+  constexpr int UN = MT + 2 * NT <= 5 ? 4 : 2;       // chunks on their way per warp, side by side
+  __shared__ float part[kSkinnyWarps][16 * NT][8 * MT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * 16;
-  const bool in0 = n0 + g < p.N, in1 = n0 + g + 8 < p.N;
-  const uint16_t* w0 = p.W + static_cast<int64_t>(in0 ? n0 + g : 0) * p.ldw;
-  const uint16_t* w1 = p.W + static_cast<int64_t>(in1 ? n0 + g + 8 : 0) * p.ldw;
+  const int n0 = blockIdx.x * 16 * NT;
+  const uint16_t* w[2 * NT];
+  bool inw[2 * NT];
+#pragma unroll
+  for (int i = 0; i < 2 * NT; ++i) {
+    inw[i] = n0 + 8 * i + g < p.N;
+    w[i] = p.W + static_cast<int64_t>(min(n0 + 8 * i + g, p.N - 1)) * p.ldw;
+  }
   const uint16_t* x[MT];
   bool inx[MT];
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
     inx[j] = 8 * j + g < p.M;
-    x[j] = p.X + static_cast<int64_t>(inx[j] ? 8 * j + g : 0) * p.ldx;
+    x[j] = p.X + static_cast<int64_t>(min(8 * j + g, p.M - 1)) * p.ldx;
   }
-  float acc[MT][4];
+  float acc[NT][MT][4];
 #pragma unroll
-  for (int j = 0; j < MT; ++j)
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
   const int chunks = (p.K + 31) / 32;
-  for (int c = warp; c < chunks; c += kSkinnyWarps * UN) {
-    uint4 a[UN], b[UN], xv[UN][MT];
+  for (int c = warp * UN; c < chunks; c += kSkinnyWarps * UN) {
+    uint4 a[UN][2 * NT], xv[UN][MT];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      const int k = (c + u * kSkinnyWarps) * 32 + t * 8;
-      a[u] = row8(w0, k, p.K, in0);
-      b[u] = row8(w1, k, p.K, in1);
+      const int k = (c + u) * 32 + t * 8;
+#pragma unroll
+      for (int i = 0; i < 2 * NT; ++i) a[u][i] = row8(w[i], k, p.K, inw[i]);
 #pragma unroll
       for (int j = 0; j < MT; ++j) xv[u][j] = row8(x[j], k, p.K, inx[j]);
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        mma16816<BF16>(acc[j], a[u].x, b[u].x, a[u].y, b[u].y, xv[u][j].x, xv[u][j].y);
-        mma16816<BF16>(acc[j], a[u].z, b[u].z, a[u].w, b[u].w, xv[u][j].z, xv[u][j].w);
-      }
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          const uint4 &lo = a[u][2 * i], &hi = a[u][2 * i + 1];
+          mma16816<BF16>(acc[i][j], lo.x, hi.x, lo.y, hi.y, xv[u][j].x, xv[u][j].y);
+          mma16816<BF16>(acc[i][j], lo.z, hi.z, lo.w, hi.w, xv[u][j].z, xv[u][j].w);
+        }
   }
   // accumulator element (row g or g + 8 of W, row 2t or 2t + 1 of x)
 #pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    part[warp][g][8 * j + 2 * t] = acc[j][0];
-    part[warp][g][8 * j + 2 * t + 1] = acc[j][1];
-    part[warp][g + 8][8 * j + 2 * t] = acc[j][2];
-    part[warp][g + 8][8 * j + 2 * t + 1] = acc[j][3];
-  }
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      part[warp][16 * i + g][8 * j + 2 * t] = acc[i][j][0];
+      part[warp][16 * i + g][8 * j + 2 * t + 1] = acc[i][j][1];
+      part[warp][16 * i + g + 8][8 * j + 2 * t] = acc[i][j][2];
+      part[warp][16 * i + g + 8][8 * j + 2 * t + 1] = acc[i][j][3];
+    }
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * 8 * MT; i += 32 * kSkinnyWarps) {
-    const int n = i & 15, m = i >> 4;
+  for (int i = threadIdx.x; i < 16 * NT * 8 * MT; i += 32 * kSkinnyWarps) {
+    const int n = i % (16 * NT), m = i / (16 * NT);
     const int row = min(m, p.M - 1), col = min(n0 + n, p.N - 1);
     const float add = from_bits<BF16>(__ldg(p.bias + static_cast<int64_t>(col) * p.bias_step));
     const float res = from_bits<BF16>(__ldg(p.residual + static_cast<int64_t>(row) * p.ldr + static_cast<int64_t>(col) * p.res_step));
     float z = 0.f;
 #pragma unroll
-    for (int w = 0; w < kSkinnyWarps; ++w) z += part[w][n][m];
+    for (int k = 0; k < kSkinnyWarps; ++k) z += part[k][n][m];
     z += p.bias_step ? add : 0.f;
     float y = z;
     switch (p.act) {
@@ -590,6 +602,7 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const SkinnyP
 
 template <int CG, int BN, int STAGES, bool PARTIAL>
 int launch_tiles(const CUtensorMap* maps, LinearParams p, cudaStream_t stream) {
+  constexpr int kEpiWarps = epi_warps<BN>;
   constexpr int SMEM = STAGES * (128 + BN / CG) * kRowBytes + kEpiWarps * 2 * 4096 + 8 * (2 * STAGES + 4) + 16 + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
   auto kernel = linear_kernel<CG, BN, STAGES, PARTIAL>;
@@ -599,7 +612,7 @@ int launch_tiles(const CUtensorMap* maps, LinearParams p, cudaStream_t stream) {
   B200S_CUDA_OK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return B200S_ERR_NO_DEVICE;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(64 + 32 * kEpiWarps);
   cfg.dynamicSmemBytes = SMEM;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -638,19 +651,25 @@ template <bool PARTIAL>
 int launch_plan(const LinearPlan& plan, const CUtensorMap* maps, const LinearParams& p, cudaStream_t stream) {
   if (plan.cta_group == 2 && plan.tile_n == 256) return launch_tiles<2, 256, 5, PARTIAL>(maps, p, stream);
   if (plan.cta_group == 2) return launch_tiles<2, 128, 6, PARTIAL>(maps, p, stream);
-  return launch_tiles<1, 128, 5, PARTIAL>(maps, p, stream);
+  if (plan.tile_n == 128) return launch_tiles<1, 128, 5, PARTIAL>(maps, p, stream);
+  return launch_tiles<1, 64, 7, PARTIAL>(maps, p, stream);
 }
 
-template <int MT>
-int launch_skinny(const SkinnyParams& p, bool bf16, cudaStream_t stream) {
-  const unsigned grid = static_cast<unsigned>((p.N + 15) / 16);
+template <int MT, int NT>
+int launch_skinny_form(const SkinnyParams& p, bool bf16, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT));
   if (bf16)
-    skinny_kernel<MT, true><<<grid, 32 * kSkinnyWarps, 0, stream>>>(p);
+    skinny_kernel<MT, NT, true><<<grid, 32 * kSkinnyWarps, 0, stream>>>(p);
   else
-    skinny_kernel<MT, false><<<grid, 32 * kSkinnyWarps, 0, stream>>>(p);
+    skinny_kernel<MT, NT, false><<<grid, 32 * kSkinnyWarps, 0, stream>>>(p);
   B200S_CUDA_OK(cudaGetLastError());
   count_launch();
   return B200S_OK;
+}
+// 32 outputs a block (each reads all of x) where that still leaves most SMs a block.
+template <int MT>
+int launch_skinny(const SkinnyParams& p, bool bf16, cudaStream_t stream) {
+  return p.N >= 32 * 120 ? launch_skinny_form<MT, 2>(p, bf16, stream) : launch_skinny_form<MT, 1>(p, bf16, stream);
 }
 
 bool tma_rows(const void* p, int64_t ld, int64_t rows) {
@@ -670,7 +689,7 @@ LinearPlan plan_linear(int64_t M, int64_t N, int64_t K, int a_major, int b_major
   // their traffic and a second launch.
   const int64_t kb = (K + kBK - 1) / kBK;
   double least = 0;
-  const struct { int cg, bn; } shapes[] = {{2, 256}, {2, 128}, {1, 128}};
+  const struct { int cg, bn; } shapes[] = {{2, 256}, {2, 128}, {1, 128}, {1, 64}};
   for (const auto& s : shapes) {
     const int64_t tiles = ((M + 128 * s.cg - 1) / (128 * s.cg)) * ((N + s.bn - 1) / s.bn);
     const int64_t units = 148 / s.cg;
