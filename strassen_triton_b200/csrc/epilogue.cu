@@ -95,18 +95,17 @@ __global__ void __launch_bounds__(kThreads) pad_rows_kernel(const uint16_t* in, 
                                                             int64_t ld_out) {
   using P = Pack<uint16_t, VEC>;
   constexpr int B = 4;
-  const int64_t per = cols / VEC, total = rows * per, step = static_cast<int64_t>(gridDim.x) * kThreads;
-  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i0 < total; i0 += B * step) {
-    P v[B];
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const uint16_t* from = in + r * ld_in;
+    uint16_t* to = out + r * ld_out;
+    for (int64_t c0 = threadIdx.x * VEC; c0 < cols; c0 += B * kThreads * VEC) {
+      P v[B];
 #pragma unroll
-    for (int b = 0; b < B; ++b) {
-      const int64_t i = i0 + b * step;
-      if (i < total) v[b] = row::ld<P>(in + (i / per) * ld_in + (i % per) * VEC);
-    }
+      for (int b = 0; b < B; ++b)
+        if (c0 + b * kThreads * VEC < cols) v[b] = row::ld<P>(from + c0 + b * kThreads * VEC);
 #pragma unroll
-    for (int b = 0; b < B; ++b) {
-      const int64_t i = i0 + b * step;
-      if (i < total) row::st(out + (i / per) * ld_out + (i % per) * VEC, v[b]);
+      for (int b = 0; b < B; ++b)
+        if (c0 + b * kThreads * VEC < cols) row::st(to + c0 + b * kThreads * VEC, v[b]);
     }
   }
 }
@@ -125,7 +124,7 @@ struct EpilogueBwd {
 template <typename T, int ACT, int VEC>
 __global__ void __launch_bounds__(kThreads) epilogue_bwd_kernel(const EpilogueBwd p) {
   using P = Pack<T, VEC>;
-  constexpr int R = VEC == 8 ? 2 : 4;      // rows on their way per thread
+  constexpr int R = 4;      // rows on their way per thread
   __shared__ float sb[8][32 * VEC + 1];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + tx) * VEC;
@@ -149,12 +148,23 @@ __global__ void __launch_bounds__(kThreads) epilogue_bwd_kernel(const EpilogueBw
         const int64_t r = r0 + k * step;
         if (r < p.M) {
           P out;
+          if constexpr (VEC >= 2 && sizeof(T) == 2) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            float v = to_f(g[k].e[e]);
-            if constexpr (ACT != B200S_ACT_NONE) v *= dact_of<T, ACT>(to_f(z[k].e[e]));
-            a[e] += v;
-            out.e[e] = from_f<T>(v);
+            for (int e = 0; e < VEC; e += 2) {
+              float2 v = row::load2(g[k].e + e);
+              if constexpr (ACT != B200S_ACT_NONE) v = row::mul_(v, epi::dact_fast2<ACT>(row::load2(z[k].e + e)));
+              a[e] += v.x;
+              a[e + 1] += v.y;
+              row::store2(out.e + e, v);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              float v = to_f(g[k].e[e]);
+              if constexpr (ACT != B200S_ACT_NONE) v *= dact_of<T, ACT>(to_f(z[k].e[e]));
+              a[e] += v;
+              out.e[e] = from_f<T>(v);
+            }
           }
           if (p.dz) row::st(static_cast<T*>(p.dz) + r * p.lddz + c, out);
         }
@@ -426,8 +436,7 @@ static int operand_rows(const void** p, int64_t* ld, int64_t rows, int64_t cols,
   uint16_t* out = reinterpret_cast<uint16_t*>(*scratch);
   const int64_t to = padded(cols);
   const bool pairs = cols % 2 == 0 && aligned(in, *ld, rows, 2, 4);
-  const int64_t blocks = (rows * cols / (pairs ? 2 : 1) + 4 * kThreads - 1) / (4 * kThreads);
-  const unsigned grid = static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16);
+  const unsigned grid = static_cast<unsigned>(rows < 148 * 16 ? rows : 148 * 16);
   if (pairs)
     pad_rows_kernel<2><<<grid, kThreads, 0, stream>>>(in, out, rows, cols, *ld, to);
   else

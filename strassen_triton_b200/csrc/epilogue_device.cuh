@@ -140,6 +140,29 @@ __device__ __forceinline__ float dact_fast(float z) {
   return dact<ACT>(z);
 }
 
+template <int ACT>
+__device__ __forceinline__ float2 dact_fast2(float2 z) {
+  using row::fma_;
+  using row::mul_;
+  if constexpr (ACT == B200S_ACT_GELU) {
+    const float2 a = make_float2(fminf(fabsf(z.x), 30.f), fminf(fabsf(z.y), 30.f));
+    const float2 h = mul_(mul_(a, a), pair(-kHalfLog2e));
+    const float2 d = fma_(a, pair(0.35f), pair(1.f));
+    const float2 t = make_float2(rcp(d.x), rcp(d.y));
+    float2 q = fma_(t, pair(-0.10458728923f), pair(0.29827082271f));
+    q = fma_(q, t, pair(-0.00994253091f));
+    q = fma_(q, t, pair(0.18356833940f));
+    q = fma_(q, t, pair(0.13218160375f));
+    q = fma_(q, t, pair(0.00050789281f));
+    // Phi(-a) - a phi(a)
+    const float2 w = mul_(fma_(a, pair(-kPdf0), q), make_float2(ex2(h.x), ex2(h.y)));
+    const float2 r = make_float2(z.x < 0.f ? w.x : 1.f - w.x, z.y < 0.f ? w.y : 1.f - w.y);
+    return make_float2(z.x == z.x ? r.x : z.x, z.y == z.y ? r.y : z.y);
+  } else {
+    return make_float2(dact_fast<ACT>(z.x), dact_fast<ACT>(z.y));
+  }
+}
+
 // f(std::integral_constant<int, ACT>) for the activation known at run time.
 template <int N>
 struct Act {

@@ -7,7 +7,7 @@
 //                   other one through the epilogue: bias, activation, residual, staging in shared memory,
 //                   TMA stores. Tile shapes 256 x 256 and 256 x 128 (CTA pairs), 128 x 128, 128 x 64; K may be cut into
 //                   parts whose fp32 partial products a second pass adds up (plan_linear weighs all this).
-//   skinny_kernel   up to 32 rows of A (tokens being generated) against K-major weights: bound by reading the
+//   skinny_kernel   up to 16 rows of A (tokens being generated) against K-major weights: bound by reading the
 //                   weights once, with mma.sync fed straight from global memory in registers.
 //
 // What bounds linear_kernel: tensor cores and the L2 reads of operand tiles; with K below about 1000 the
@@ -666,10 +666,10 @@ int launch_skinny_form(const SkinnyParams& p, bool bf16, cudaStream_t stream) {
   count_launch();
   return B200S_OK;
 }
-// 32 outputs a block (each reads all of x) where that still leaves most SMs a block.
+// 32 outputs a block where that still leaves most SMs a block (1 x 8192 x 8192: 27 us against 33 with 16).
 template <int MT>
 int launch_skinny(const SkinnyParams& p, bool bf16, cudaStream_t stream) {
-  return p.N >= 32 * 120 ? launch_skinny_form<MT, 2>(p, bf16, stream) : launch_skinny_form<MT, 1>(p, bf16, stream);
+  return MT == 1 && p.N >= 32 * 120 ? launch_skinny_form<1, 2>(p, bf16, stream) : launch_skinny_form<MT, 1>(p, bf16, stream);
 }
 
 bool tma_rows(const void* p, int64_t ld, int64_t rows) {
@@ -680,25 +680,31 @@ bool tma_rows(const void* p, int64_t ld, int64_t rows) {
 
 LinearPlan plan_linear(int64_t M, int64_t N, int64_t K, int a_major, int b_major) {
   LinearPlan best{LinearPlan::kTiles, 2, 256, 1};
-  if (M <= 32 && a_major == B200S_K_MAJOR && b_major == B200S_K_MAJOR) {
+  // Few rows: the weights are read once, as fast as by a copy (16 x 4096 x 4096: 9.4 us; tiles take 11). With 32
+  // rows a block's reading of x costs more than the weights (15.4 us against 11.1 with tiles).
+  if (M <= 16 && a_major == B200S_K_MAJOR && b_major == B200S_K_MAJOR) {
     best.kind = LinearPlan::kSkinny;
     return best;
   }
-  // Estimated clocks of every tile shape and split: waves of tiles, each bound by the tensor cores (4096
-  // products a clock and SM) or by reading operands from L2 (60 bytes a clock and SM); partial products cost
-  // their traffic and a second launch.
+  // Estimated clocks of every tile shape and split. Measured, per 64 of K: 540 clocks for one CTA (its TMA
+  // loads), 680 for a pair, never less than the tensor cores need (4096 products a clock and SM), and with all
+  // SMs loading 45 bytes a clock and SM from L2; 4.0 and 5.4 us for a launch with one such step. A split adds
+  // the pass over the partial products (2.3 us and its traffic, slower where rows are not whole vectors).
   const int64_t kb = (K + kBK - 1) / kBK;
   double least = 0;
   const struct { int cg, bn; } shapes[] = {{2, 256}, {2, 128}, {1, 128}, {1, 64}};
   for (const auto& s : shapes) {
     const int64_t tiles = ((M + 128 * s.cg - 1) / (128 * s.cg)) * ((N + s.bn - 1) / s.bn);
     const int64_t units = 148 / s.cg;
-    const double mma = s.bn / s.cg * s.cg * 0.5 * 4, fill = (128.0 + s.bn / s.cg) * kRowBytes / 60.0;
+    const double mma = s.bn * 2.0, bytes = (128.0 + s.bn / s.cg) * kRowBytes;
     for (int split = 1; split <= 16 && split <= kb; ++split) {
-      const int64_t waves = (tiles * split + units - 1) / units;
-      const double tile = static_cast<double>((kb + split - 1) / split) * (mma > fill ? mma : fill) + 800;
-      double clocks = static_cast<double>(waves) * tile + 2500;
-      if (split > 1) clocks += 4500 + static_cast<double>(M) * static_cast<double>(N) * (8.0 * split + 2) / 4500;
+      const int64_t work = tiles * split, waves = (work + units - 1) / units;
+      const double busy = static_cast<double>(work < units ? work : units) / static_cast<double>(units);
+      double step = s.cg == 2 ? 680 : 540;
+      if (step < mma) step = mma;
+      if (step < bytes / 45.0 * busy) step = bytes / 45.0 * busy;
+      double clocks = (s.cg == 2 ? 10200 : 7600) + static_cast<double>(waves) * static_cast<double>((kb + split - 1) / split) * step;
+      if (split > 1) clocks += 4400 + static_cast<double>(M) * static_cast<double>(N) * (4.0 * split + 2) / (N % 4 == 0 ? 2400 : 900);
       if (least == 0 || clocks < least) {
         least = clocks;
         best.cta_group = s.cg, best.tile_n = s.bn, best.splits = split;
@@ -721,9 +727,7 @@ int launch_linear(const LinearArgs& g, const LinearPlan& plan, cudaStream_t stre
     p.residual = g.residual ? static_cast<const uint16_t*>(g.residual) : p.X, p.res_step = g.residual ? 1 : 0;
     p.ldx = g.lda, p.ldw = g.ldb, p.ldc = g.ldc, p.ldr = g.residual ? g.ldr : 0, p.ldz = g.ldz;
     p.M = static_cast<int32_t>(g.M), p.N = static_cast<int32_t>(g.N), p.K = static_cast<int32_t>(g.K), p.act = g.activation;
-    if (g.M <= 8) return launch_skinny<1>(p, bf16_out, stream);
-    if (g.M <= 16) return launch_skinny<2>(p, bf16_out, stream);
-    return launch_skinny<4>(p, bf16_out, stream);
+    return g.M <= 8 ? launch_skinny<1>(p, bf16_out, stream) : launch_skinny<2>(p, bf16_out, stream);
   }
   const bool partial = plan.splits > 1;
   uint32_t* status = device_status_words();
