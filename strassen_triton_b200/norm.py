@@ -81,10 +81,10 @@ def _backward(dy, x, weight, st, param_dtype, need_x, need_w, need_b):
     ws, need = None, 0
     if need_w or need_b:
         need = _workspace_bytes(rows, d)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr()     # freed and reused in stream order
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)     # held until the launch
     mean = st.data_ptr()
     call(dev, _lib.load().b200s_layer_norm_backward, rows, d, DTYPE[x.dtype], DTYPE[param_dtype], xr.data_ptr(), ldx,
-         gr.data_ptr(), ldg, ptr(w), mean, mean + 4 * rows, ptr(dx), d, ptr(dw), ptr(db), ws, need)
+         gr.data_ptr(), ldg, ptr(w), mean, mean + 4 * rows, ptr(dx), d, ptr(dw), ptr(db), ptr(ws), need)
     return dx, dw, db
 
 

@@ -443,10 +443,11 @@ def _dense_forward(x, weight, bias, residual, act, save):
         rp, ldr = residual.data_ptr(), residual.stride(0)
     code = _DTYPE[dt]
     need = _dense_workspace(False, M, N, K, code, 0, 1 if _off_grid(x) or _off_grid(weight) else 0)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr() if need else None     # reused in stream order
+    # held until the launch: freed, it could go to another thread's call on this stream before that
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _call.call(dev, _lib.load().b200s_linear_act, M, N, K, code, act, x.data_ptr(), x.stride(0), weight.data_ptr(),
                weight.stride(0), None if bias is None else bias.data_ptr(), rp, ldr, y.data_ptr(), N,
-               None if z is None else z.data_ptr(), ldz, ws, need)
+               None if z is None else z.data_ptr(), ldz, None if ws is None else ws.data_ptr(), need)
     return y, z
 
 
@@ -462,11 +463,11 @@ def _dense_backward(dy, x, weight, z, act, need_x, need_w, need_b):
     db = torch.empty(N, dtype=dt, device=dev) if need_b else None
     code = _DTYPE[dt]
     need = _dense_workspace(True, M, N, K, code, act, 1 if _off_grid(x) or _off_grid(weight) or _off_grid(dy) else 0)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr()
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
     p = _call.ptr
     _call.call(dev, _lib.load().b200s_linear_act_backward, M, N, K, code, act, x.data_ptr(), x.stride(0), weight.data_ptr(),
                weight.stride(0), p(z), z.shape[1] if z is not None else 0, dy.data_ptr(), dy.stride(0), p(dx), K, p(dw), K,
-               p(db), ws, need)
+               p(db), ws.data_ptr(), need)
     return dx, dw, db
 
 

@@ -110,6 +110,38 @@ def test_layouts(b200s):
         check(o, s, 1 / (want + 1e-6))
 
 
+def test_more_tensors_than_one_launch_takes(b200s):
+    grads = make([5 + i % 7 for i in range(1300)], ALL)
+    want = norm64(grads)
+    out = [torch.empty_like(t, dtype=torch.float32) for t in grads]
+    n = b200s.clip_grads_(grads, want / 3, out=out)
+    assert abs(n.item() / want - 1) < 2.0 ** -22 and torch.equal(n, b200s.grad_norm(grads))
+    for o, t in zip(out, grads):
+        check(o, t, (want / 3) / (want + 1e-6))
+
+
+def test_shards_of_several_ranks(b200s, monkeypatch):
+    """With a process group the sums of squares of all ranks are added before the root: here a second rank that holds
+    three times the squares."""
+    import torch.distributed as dist
+
+    seen = []
+
+    def all_reduce(t, group=None):
+        seen.append(group)
+        t.mul_(4.0)
+
+    monkeypatch.setattr(dist, "all_reduce", all_reduce)
+    grads = make([100, 33], [torch.float32])
+    want = 2 * norm64(grads)
+    keep = [t.clone() for t in grads]
+    assert abs(b200s.grad_norm(grads, group="shards").item() / want - 1) < 2.0 ** -22
+    n = b200s.clip_grads_(grads, want / 2, group="shards")
+    assert abs(n.item() / want - 1) < 2.0 ** -22 and seen == ["shards", "shards"]
+    for a, t in zip(grads, keep):
+        check(a, t, (want / 2) / (want + 1e-6))
+
+
 def test_extreme_and_nonfinite_values(b200s):
     """Squares are fp64: neither 1e30 nor 1e-30 is lost. inf makes the coefficient zero, NaN makes everything NaN."""
     for scale in (1e30, 1e-30):

@@ -73,7 +73,7 @@ def inputs(rows, d, dtype, wdtype, seed=0, shift=0.5):
     return x, (1 + 0.1 * r(d)).to(wdtype), (0.1 * r(d)).to(wdtype), r(rows, d).to(dtype)
 
 
-SHAPES = [(1, 1), (1, 768), (3, 7), (5, 33), (2, 255), (64, 256), (37, 768), (300, 1024), (9, 1601), (33, 4096), (8, 4104),
+SHAPES = [(700, 2048), (500, 5000), (310, 16384), (460, 4096), (20, 20000), (900, 1030), (1, 1), (1, 768), (3, 7), (5, 33), (2, 255), (64, 256), (37, 768), (300, 1024), (9, 1601), (33, 4096), (8, 4104),
           (5, 8192), (3, 12289), (2, 40000), (1000, 64), (2049, 48), (1, 2), (17, 96), (130, 2304)]
 
 

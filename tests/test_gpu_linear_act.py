@@ -253,6 +253,50 @@ def test_graphs_streams_and_repeats(b200s, m):
         assert all(torch.equal(p, q) for p, q in zip(a, c))
 
 
+def test_two_threads_on_one_stream(b200s):
+    """Calls from two host threads share the stream and the allocator: each keeps its own scratch and results."""
+    import threading
+
+    cases = [inputs(300, 515, 770, torch.bfloat16, seed=s) for s in (1, 2)]
+
+    def step(c):
+        x, w, b, r, dy = c
+        v = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        y = b200s.linear_act(*v, "gelu", r)
+        return [y.detach()] + list(torch.autograd.grad(y, v, dy))
+
+    want = [step(c) for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        for _ in range(40):
+            got = step(cases[k])
+            if not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                bad.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_offsets_past_32_bits(b200s):
+    """A result of more than 2^31 elements (4.3 GB), stored by TMA and, with rows of odd length, element by element."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for m, n in ((66000, 32768), (70001, 30721)):
+        x = torch.zeros(m, 16, device="cuda", dtype=torch.bfloat16)
+        x[-3:] = torch.randn(3, 16, generator=g, device="cuda").bfloat16()
+        w = torch.randn(n, 16, generator=g, device="cuda").bfloat16()
+        y = b200s.linear_act(x, w, None, "silu")
+        want = act64(x[-3:].double() @ w.double().t(), "silu")
+        check("last rows", y[-3:], want, 2.0 ** -15 * (1 + want.abs()), torch.bfloat16)
+        assert not y[-200:-3].any()
+        del y
+
+
 def test_linear_strassen_module(b200s):
     """LinearStrassen's activation and residual, and the plain layer left as it was."""
     from model.layers import LinearStrassen
