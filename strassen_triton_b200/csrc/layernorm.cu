@@ -15,6 +15,9 @@
 // takes, then in one row of partial sums per block, then over the blocks in their order by a second
 // kernel. VEC is 16 bytes where rows and pointers allow it, else 4 bytes, else one element. Longer rows
 // take the looping kernels, which read a row again (from L1 / L2) instead of keeping it.
+//
+// Measured: 16381 x 4096 fp16 with fp32 parameters 48 us forward (5.6 TB/s) and 76 + 4 us backward (5.3 TB/s);
+// 8192 x 768 bf16, resident in L2, 6.4 us and 12.4 + 4 us, where latency counts: a warp has one to five rows.
 
 #include <cuda_runtime.h>
 
@@ -489,7 +492,8 @@ norm_bwd_kernel(const NormBwd p) {
 
 // ---- rows of a block fed through shared memory -------------------------------------------------
 // The block-per-row forms read a row, meet at a barrier, and only then finish it: with one row in
-// flight per block HBM waits for the barriers (d = 4096, 16-bit: 2.4 TB/s read by the backward pass).
+// flight per block HBM waits for the barriers (d = 4096, 16-bit, backward: 112 us, here 97; 76 with 16 elements
+// a thread instead of 8 and cheaper trees of sums, 109 with 32 on 128 threads).
 // Here one thread keeps `stages` rows on their way into shared memory with bulk copies, whatever the
 // other threads wait for. A stage is free again after the barrier of its row's sums, which every thread
 // reaches after reading it. Waits are bounded: a block that gives up lets its copies land, reports and

@@ -4,14 +4,17 @@
 // Two kernels:
 //   linear_kernel   tcgen05 tiles. Warp 0 loads 128-byte-swizzled operand tiles by TMA, one lane of warp 1
 //                   issues tcgen05.mma into one of two accumulators in tensor memory, warps 2.. take the
-//                   other one through the epilogue: bias, activation, residual, staging in shared memory,
-//                   TMA stores. Tile shapes 256 x 256 and 256 x 128 (CTA pairs), 128 x 128, 128 x 64; K may be cut into
+//                   other one through the epilogue: bias, activation, residual, rows of results through
+//                   shared memory. Tile shapes 256 x 256 and 256 x 128 (CTA pairs), 128 x 128, 128 x 64; K may be cut into
 //                   parts whose fp32 partial products a second pass adds up (plan_linear weighs all this).
 //   skinny_kernel   up to 16 rows of A (tokens being generated) against K-major weights: bound by reading the
 //                   weights once, with mma.sync fed straight from global memory in registers.
 //
-// What bounds linear_kernel: tensor cores and the L2 reads of operand tiles; with K below about 1000 the
-// epilogue's arithmetic comes close to the product's (a GELU is 11 instructions and two of the 16-a-clock unit).
+// What bounds linear_kernel: L2 reads of operand tiles. A 256 x 256 pair reads 64 KB per 64 of K, and with all
+// SMs loading the steps come 0.39 .. 0.48 us apart, about 12 TB/s, where the tensor cores need 0.27. (A library
+// product that shares tiles between clusters by multicast, which this package does without, takes 337 us for
+// 8192 x 4096 x 8192 where this kernel takes 374 and with GELU and bias 389.) With K below about 1000 the epilogue's
+// arithmetic adds to it: 8192 x 768 -> 2304 takes 28 us plain, 37 with GELU and bias, 41 with z stored too.
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -45,8 +48,7 @@ struct LinearParams {
   int32_t raster_group;
   int32_t a_mn, b_mn, fmt;
   int32_t bf16_out, act;
-  int32_t tma_c, tma_z;          // results that TMA can store
-  int32_t vec_r;                 // residual rows are 16-byte aligned
+  int32_t vec_c, vec_z, vec_r;   // C, Z, the residual: rows of whole, aligned 16-byte vectors
   const void* bias;
   const void* residual;
   void* C;
@@ -102,32 +104,41 @@ __device__ __forceinline__ void activate(float2 (&v)[32], int act) {
   }
 }
 
-// One warp's 32 x 64 block of 16-bit results, packed by its lanes (lane = row), goes through a swizzled 4 KB
-// buffer to row0, col0 of a matrix: by TMA, or row by row where TMA cannot address the matrix.
-__device__ __forceinline__ void store_block(const CUtensorMap* map, bool tma, void* dst, int64_t ld, int M, int N, int row0, int col0,
+// One warp's block of 32 rows x 128 bytes, written by its lanes (lane = row) into a swizzled 4 KB buffer, goes to
+// row0, byte column col0 of a matrix of `rows` rows of `row_bytes` bytes, `ld` bytes apart: 16 bytes a lane where the
+// rows are whole aligned vectors, else 2 bytes a lane. (With TMA stores instead, two buffers a warp and a stage
+// fewer for the operands, 8192 x 4096 -> 8192 with relu2, bias and residual took 519 us back to back, 488 so.)
+__device__ __forceinline__ void store_block(uint8_t* dst, int64_t ld, bool vec, int rows, int64_t row_bytes, int row0, int64_t col0,
                                             uint32_t buf, const uint32_t (&h)[32], int lane) {
   const uint32_t srow = buf + static_cast<uint32_t>(lane) * 128u, sw = static_cast<uint32_t>(lane & 7);
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     ptx::st_shared_v4(srow + ((static_cast<uint32_t>(j) ^ sw) << 4), h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
-  if (tma) {
-    ptx::fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) ptx::tma_store_3d(map, buf, col0, row0, 0);
-    return;
-  }
   __syncwarp();
-  unsigned short* out = static_cast<unsigned short*>(dst);
-  const int rows = min(32, M - row0), cols = N - col0;
-  for (int r = 0; r < rows; ++r) {
+  uint8_t* at = dst + static_cast<int64_t>(row0) * ld + col0;
+  const int n = min(32, rows - row0);
+  const int64_t left = row_bytes - col0;
+  if (vec) {
+    const int q = lane >> 3, c = (lane & 7) * 16;
+    if (c < left) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int c = lane + 32 * k;
-      uint16_t v;
-      asm volatile("ld.shared.u16 %0, [%1];"
-                   : "=h"(v)
-                   : "r"(buf + static_cast<uint32_t>(r) * 128u + ((static_cast<uint32_t>(c >> 3) ^ static_cast<uint32_t>(r & 7)) << 4) + (c & 7) * 2u));
-      if (c < cols) out[static_cast<int64_t>(row0 + r) * ld + col0 + c] = v;
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + q;
+        const uint4 v = ptx::ld_shared_v4(buf + static_cast<uint32_t>(r) * 128u + ((static_cast<uint32_t>(lane & 7) ^ static_cast<uint32_t>(r & 7)) << 4));
+        if (r < n) *reinterpret_cast<uint4*>(at + r * ld + c) = v;
+      }
+    }
+  } else {
+    for (int r = 0; r < n; ++r) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int c = lane + 32 * k;
+        uint16_t v;
+        asm volatile("ld.shared.u16 %0, [%1];"
+                     : "=h"(v)
+                     : "r"(buf + static_cast<uint32_t>(r) * 128u + ((static_cast<uint32_t>(c >> 3) ^ static_cast<uint32_t>(r & 7)) << 4) + (c & 7) * 2u));
+        if (2 * c < left) *reinterpret_cast<uint16_t*>(at + r * ld + 2 * c) = v;
+      }
     }
   }
   __syncwarp();
@@ -135,15 +146,14 @@ __device__ __forceinline__ void store_block(const CUtensorMap* map, bool tma, vo
 
 template <int CG, int BN, int STAGES, bool PARTIAL>
 __global__ void __launch_bounds__(64 + 32 * epi_warps<BN>, 1)
-linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
-              const __grid_constant__ CUtensorMap tmZ, const LinearParams p) {
+linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const LinearParams p) {
   constexpr int kEpiWarps = epi_warps<BN>;
   constexpr int BN_CTA = BN / CG;
   constexpr int A_BYTES = 128 * kRowBytes;
   constexpr int B_BYTES = BN_CTA * kRowBytes;
   constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   constexpr int CHUNK_BYTES = kBK * kRowBytes;       // an MN-major chunk: 64 k-rows of 64 elements
-  constexpr int STAGING = kEpiWarps * 2 * 4096;
+  constexpr int STAGING = kEpiWarps * 4096;
   constexpr uint32_t TMEM_COLS = 2 * BN;
 
   extern __shared__ uint8_t smem_raw[];
@@ -176,8 +186,6 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     ptx::fence_mbar_init();
     ptx::prefetch_tensormap(&tmA);
     ptx::prefetch_tensormap(&tmB);
-    if (p.tma_c) ptx::prefetch_tensormap(&tmC);
-    if (p.tma_z) ptx::prefetch_tensormap(&tmZ);
   }
   if (warp == 1) {
     ptx::tmem_alloc<CG>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), TMEM_COLS);
@@ -285,20 +293,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     const int lane_group = warp & 3;        // this warp's TMEM lanes [32 * lane_group, +32)
     const int half = ew >> 2;               // and share of the tile's columns
     constexpr int WN = BN / (kEpiWarps / 4);
-    const uint32_t stg = staging + static_cast<uint32_t>(ew) * 8192u;
+    const uint32_t b = staging + static_cast<uint32_t>(ew) * 4096u;    // this warp's buffer
     const bool bf16 = p.bf16_out != 0;
-    int flip = 0, it = 0;
-    // the next staging buffer, once the store that last read it is done with it
-    auto next_buffer = [&]() {
-      const uint32_t b = stg + static_cast<uint32_t>(flip) * 4096u;
-      flip ^= 1;
-      if (lane == 0) ptx::tma_store_wait_read<1>();
-      __syncwarp();
-      return b;
-    };
-    auto sent = [&]() {      // every buffer is one bulk group, stored by TMA or not
-      if (lane == 0) ptx::tma_store_commit();
-    };
+    int it = 0;
     for (int tile = cluster; tile < p.total_tiles; tile += clusters, ++it) {
       const Tile t = decode(p, tile);
       const int buf = it & 1;
@@ -356,19 +353,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         }
         if (col0 >= p.N || row0 >= p.M) continue;
         if constexpr (PARTIAL) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t b = next_buffer();
-            const uint32_t srow = b + static_cast<uint32_t>(lane) * 128u, sw = static_cast<uint32_t>(lane & 7);
-            const uint32_t(&r)[32] = h == 0 ? r0 : r1;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              ptx::st_shared_v4(srow + ((static_cast<uint32_t>(j) ^ sw) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0 && col0 + 32 * h < p.N) ptx::tma_store_3d(&tmC, b, col0 + 32 * h, row0, t.split);
-            sent();
-          }
+          uint8_t* dst = static_cast<uint8_t*>(p.C) + static_cast<int64_t>(t.split) * p.M * p.ldc * 4;
+          store_block(dst, p.ldc * 4, true, p.M, p.ldc * 4, row0, static_cast<int64_t>(col0) * 4, b, r0, lane);
+          if (col0 + 32 < p.N) store_block(dst, p.ldc * 4, true, p.M, p.ldc * 4, row0, static_cast<int64_t>(col0 + 32) * 4, b, r1, lane);
         } else {
           float2 v[32];
 #pragma unroll
@@ -387,11 +374,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           if (p.Z != nullptr) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) h[j] = pack2(v[j].x, v[j].y, bf16);
-            store_block(&tmZ, p.tma_z != 0, p.Z, p.ldz, p.M, p.N, row0, col0, next_buffer(), h, lane);
-            sent();
+            store_block(static_cast<uint8_t*>(p.Z), p.ldz * 2, p.vec_z != 0, p.M, static_cast<int64_t>(p.N) * 2, row0, static_cast<int64_t>(col0) * 2, b, h, lane);
           }
           activate(v, p.act);
-          const uint32_t b = next_buffer();
           if (p.residual != nullptr) {
             // rows as they were read -> rows of the lanes, through the buffer the result will use
             if (vec_res) {
@@ -428,13 +413,10 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j) h[j] = pack2(v[j].x, v[j].y, bf16);
-          store_block(&tmC, p.tma_c != 0, p.C, p.ldc, p.M, p.N, row0, col0, b, h, lane);
-          sent();
+          store_block(static_cast<uint8_t*>(p.C), p.ldc * 2, p.vec_c != 0, p.M, static_cast<int64_t>(p.N) * 2, row0, static_cast<int64_t>(col0) * 2, b, h, lane);
         }
       }
     }
-    if (lane == 0) ptx::tma_store_wait_all<0>();     // shared memory must outlive the stores
-    __syncwarp();
   }
 
   // ------------------------------------------------------------ teardown
@@ -603,7 +585,7 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const SkinnyP
 template <int CG, int BN, int STAGES, bool PARTIAL>
 int launch_tiles(const CUtensorMap* maps, LinearParams p, cudaStream_t stream) {
   constexpr int kEpiWarps = epi_warps<BN>;
-  constexpr int SMEM = STAGES * (128 + BN / CG) * kRowBytes + kEpiWarps * 2 * 4096 + 8 * (2 * STAGES + 4) + 16 + 1024;
+  constexpr int SMEM = STAGES * (128 + BN / CG) * kRowBytes + kEpiWarps * 4096 + 8 * (2 * STAGES + 4) + 16 + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
   auto kernel = linear_kernel<CG, BN, STAGES, PARTIAL>;
   static std::mutex mu;
@@ -642,17 +624,17 @@ int launch_tiles(const CUtensorMap* maps, LinearParams p, cudaStream_t stream) {
   if (fit < 1) return B200S_ERR_NO_DEVICE;
   cfg.gridDim = dim3((p.total_tiles < fit ? p.total_tiles : fit) * CG);
   cfg.stream = stream;
-  B200S_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], p));
+  B200S_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], p));
   count_launch();
   return B200S_OK;
 }
 
 template <bool PARTIAL>
 int launch_plan(const LinearPlan& plan, const CUtensorMap* maps, const LinearParams& p, cudaStream_t stream) {
-  if (plan.cta_group == 2 && plan.tile_n == 256) return launch_tiles<2, 256, 5, PARTIAL>(maps, p, stream);
-  if (plan.cta_group == 2) return launch_tiles<2, 128, 6, PARTIAL>(maps, p, stream);
-  if (plan.tile_n == 128) return launch_tiles<1, 128, 5, PARTIAL>(maps, p, stream);
-  return launch_tiles<1, 64, 7, PARTIAL>(maps, p, stream);
+  if (plan.cta_group == 2 && plan.tile_n == 256) return launch_tiles<2, 256, 6, PARTIAL>(maps, p, stream);
+  if (plan.cta_group == 2) return launch_tiles<2, 128, 7, PARTIAL>(maps, p, stream);
+  if (plan.tile_n == 128) return launch_tiles<1, 128, 6, PARTIAL>(maps, p, stream);
+  return launch_tiles<1, 64, 8, PARTIAL>(maps, p, stream);
 }
 
 template <int MT, int NT>
@@ -672,7 +654,7 @@ int launch_skinny(const SkinnyParams& p, bool bf16, cudaStream_t stream) {
   return MT == 1 && p.N >= 32 * 120 ? launch_skinny_form<1, 2>(p, bf16, stream) : launch_skinny_form<MT, 1>(p, bf16, stream);
 }
 
-bool tma_rows(const void* p, int64_t ld, int64_t rows) {
+bool vector_rows(const void* p, int64_t ld, int64_t rows) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (rows <= 1 || (ld * 2) % 16 == 0);
 }
 
@@ -732,7 +714,7 @@ int launch_linear(const LinearArgs& g, const LinearPlan& plan, cudaStream_t stre
   const bool partial = plan.splits > 1;
   uint32_t* status = device_status_words();
   if (!status) return B200S_ERR_NO_DEVICE;
-  CUtensorMap maps[4];
+  CUtensorMap maps[2];
   const int cg = plan.cta_group, bn_cta = plan.tile_n / cg;
   int rc = g.a_major == B200S_K_MAJOR ? encode_operand_map(&maps[0], g.A, g.in_dtype, g.M, g.K, g.lda, 1, 0, 128, false)
                                       : encode_operand_map(&maps[0], g.A, g.in_dtype, g.K, g.M, g.lda, 1, 0, kBK, false);
@@ -741,19 +723,10 @@ int launch_linear(const LinearArgs& g, const LinearPlan& plan, cudaStream_t stre
                                   : encode_operand_map(&maps[1], g.B, g.in_dtype, g.K, g.N, g.ldb, 1, 0, kBK, false);
   if (rc) return rc;
   LinearParams p = {};
-  maps[2] = maps[3] = maps[0];     // never used unless built below
-  if (partial) {
-    rc = encode_operand_map(&maps[2], g.partials, B200S_FP32, g.M, g.N, g.ldp, plan.splits, g.M * g.ldp, 32, true);
-    if (rc) return rc;
-    p.tma_c = 1;
-  } else {
-    p.tma_c = tma_rows(g.C, g.ldc, g.M) && g.ldc >= g.N;
-    p.tma_z = g.preact && tma_rows(g.preact, g.ldz, g.M) && g.ldz >= g.N;
-    // (a single row needs no stride of its own, but the map wants a legal one)
-    const int64_t ldc = g.M > 1 ? g.ldc : (g.N + 7) / 8 * 8, ldz = g.M > 1 ? g.ldz : (g.N + 7) / 8 * 8;
-    if (p.tma_c && (rc = encode_operand_map(&maps[2], g.C, g.out_dtype, g.M, g.N, ldc, 1, 0, 32, true)) != 0) return rc;
-    if (p.tma_z && (rc = encode_operand_map(&maps[3], g.preact, g.out_dtype, g.M, g.N, ldz, 1, 0, 32, true)) != 0) return rc;
-  }
+  const bool whole = g.N % 8 == 0;
+  p.vec_c = whole && vector_rows(g.C, g.ldc, g.M);
+  p.vec_z = g.preact && whole && vector_rows(g.preact, g.ldz, g.M);
+  p.vec_r = g.residual && whole && vector_rows(g.residual, g.ldr, g.M);
   p.M = static_cast<int32_t>(g.M), p.N = static_cast<int32_t>(g.N), p.K = static_cast<int32_t>(g.K);
   p.m_tiles = static_cast<int32_t>((g.M + 128 * cg - 1) / (128 * cg));
   p.n_tiles = static_cast<int32_t>((g.N + plan.tile_n - 1) / plan.tile_n);
@@ -768,7 +741,7 @@ int launch_linear(const LinearArgs& g, const LinearPlan& plan, cudaStream_t stre
   p.bf16_out = bf16_out, p.act = g.activation;
   p.bias = g.bias, p.residual = g.residual, p.C = g.C, p.Z = g.preact;
   p.ldc = g.ldc, p.ldr = g.ldr, p.ldz = g.ldz;
-  p.vec_r = g.residual && tma_rows(g.residual, g.ldr, g.M) && g.N % 8 == 0;
+  if (partial) p.C = g.partials, p.ldc = g.ldp;       // rows of whole vectors, the last one filled up
   p.status = status;
   return partial ? launch_plan<true>(plan, maps, p, stream) : launch_plan<false>(plan, maps, p, stream);
 }
