@@ -167,6 +167,8 @@ def clip_grads_(grads: Iterable[Tensor], max_norm: float, *, out: Optional[Seque
     call(dev, lib.b200s_grad_clip, arr.buffer_info()[0], len(grads), parts.data_ptr(), n_parts, max_norm, norm.data_ptr())
     for t, s in back:
         t.copy_(s)
+    # written behind autograd's back: whoever saved one of them for a backward pass learns of it
+    torch.autograd.graph.increment_version(grads if out is None else out)
     return norm
 
 

@@ -20,6 +20,8 @@ from . import ops
 
 
 class LinearStrassen(nn.Linear):
+    activation = "none"     # of layers pickled before they had one
+
     def __init__(self, in_features: int, out_features: Optional[int] = None, bias: bool = True, dtype=None,
                  depth: Optional[int] = 1, device="cuda", algo: str = "classic", activation: str = "none") -> None:
         # main_profiling.py:51-60 spells the constructor (features, bias, dtype, depth, device)

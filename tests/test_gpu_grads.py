@@ -187,6 +187,16 @@ def test_parameters_as_torch_does(b200s):
     assert a[1].bias.grad is None
 
 
+def test_autograd_notices_the_clipping(b200s):
+    """A gradient that a second backward pass needs may not be scaled under it silently."""
+    x = torch.ones(10, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    loss = (g ** 2).sum()
+    b200s.clip_grads_([g.detach()], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_refusals(b200s):
     g = make([10, 20], [torch.float32])
     with pytest.raises(ValueError):
