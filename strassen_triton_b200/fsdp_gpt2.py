@@ -67,6 +67,7 @@ class Block(nn.Module):
         self.out = mk(4 * d, d)       # X[8192,3072] . W[3072,768]
         if fused:
             self.fc.activation = "gelu"
+            self.qkv.one_call = True
 
     def forward(self, x):
         b, t, d = x.shape
@@ -90,6 +91,8 @@ class GPT(nn.Module):
         self.blocks = nn.ModuleList(Block(d, heads, depth, device, plain, fused) for _ in range(layers))
         self.ln_f = (LayerNorm if fused else nn.LayerNorm)(d, device=device)
         self.lm_head = _linear_factory(depth, device, plain)(d, VOCAB_PADDED)
+        if fused:
+            self.lm_head.one_call = True
         for m in self.modules():
             if isinstance(m, (nn.Linear, nn.Embedding)):
                 nn.init.normal_(m.weight, std=0.02)

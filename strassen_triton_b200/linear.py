@@ -21,6 +21,7 @@ from . import ops
 
 class LinearStrassen(nn.Linear):
     activation = "none"     # of layers pickled before they had one
+    one_call = False        # take ops.linear_act for the plain layer too (its products, and one call per direction)
 
     def __init__(self, in_features: int, out_features: Optional[int] = None, bias: bool = True, dtype=None,
                  depth: Optional[int] = 1, device="cuda", algo: str = "classic", activation: str = "none") -> None:
@@ -63,7 +64,7 @@ class LinearStrassen(nn.Linear):
                 depth -= 1
             if depth == 0:
                 algo = "dense"
-        if self.activation != "none" or residual is not None:
+        if self.activation != "none" or residual is not None or self.one_call:
             if residual is not None and residual.dtype != x.dtype:
                 residual = residual.to(x.dtype)
             if residual is not None:

@@ -471,6 +471,17 @@ def _dense_backward(dy, x, weight, z, act, need_x, need_w, need_b):
     return dx, dw, db
 
 
+def _auto_is_dense(M, N, K, code) -> bool:
+    """Does the tuner table choose the dense product for the layer and for both products of its backward pass?"""
+    lookup = _lib.load().b200s_tuner_lookup
+    a, d = ctypes.c_int32(0), ctypes.c_int32(0)
+    pa, pd = ctypes.byref(a), ctypes.byref(d)
+    for m, n, k in ((M, N, K), (M, K, N), (N, K, M)):
+        if lookup(m, n, k, code, pa, pd) or (a.value != _lib.ALGO_DENSE and d.value != 0):
+            return False
+    return True
+
+
 class _DenseLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
@@ -588,8 +599,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
             residual = residual.reshape(-1, out_shape[-1])
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     depth = int(depth)
-    if (algo == "dense" and x.dtype != torch.float32 and _rows_contiguous(x2) and _rows_contiguous(weight)
-            and not torch.compiler.is_compiling()):
+    if (x.dtype != torch.float32 and _rows_contiguous(x2) and _rows_contiguous(weight) and not torch.compiler.is_compiling()
+            and (algo == "dense" or (algo == "auto" and x2.shape[0] > 0
+                                     and _auto_is_dense(x2.shape[0], weight.shape[0], weight.shape[1], _DTYPE[x.dtype])))):
         if _call.wants_grad(x, weight, bias, residual):
             y = _DenseLinearFn.apply(x2, weight, bias, residual, act)
         else:

@@ -297,6 +297,28 @@ def test_offsets_past_32_bits(b200s):
         del y
 
 
+def test_the_table_decides_between_dense_and_strassen(b200s, tmp_path):
+    """algo "auto" follows the tuner table at every call: dense entries give the dense layer bit for bit, a Strassen
+    entry the Strassen product."""
+    from strassen_triton_b200 import _lib
+
+    lib = _lib.load()
+    keep = str(tmp_path / "table.txt").encode()
+    assert lib.b200s_tuner_save(keep) == 0
+    x, w, b, r, _ = inputs(512, 512, 512, torch.bfloat16)
+    dense = b200s.linear_act(x, w, b, "gelu", r)
+    strassen = b200s.linear_act(x, w, b, "gelu", r, algo="classic", depth=1)
+    try:
+        for algo, depth, want in ((_lib.ALGO_DENSE, 0, dense), (_lib.ALGO_CLASSIC, 1, strassen), (_lib.ALGO_DENSE, 0, dense)):
+            lib.b200s_tuner_clear()
+            assert lib.b200s_tuner_record(512, 512, 512, _lib.BF16, algo, depth) == 0
+            assert torch.equal(b200s.linear_act(x, w, b, "gelu", r, algo="auto", depth=-1), want)
+    finally:
+        lib.b200s_tuner_clear()
+        assert lib.b200s_tuner_load(keep) == 0
+    assert not torch.equal(dense, strassen)
+
+
 def test_linear_strassen_module(b200s):
     """LinearStrassen's activation and residual, and the plain layer left as it was."""
     from model.layers import LinearStrassen
