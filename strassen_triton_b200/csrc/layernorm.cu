@@ -764,8 +764,9 @@ int ring_stages(uint32_t stage_bytes, int per_sm) {
 
 template <class K>
 int allow_smem(K kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return B200S_OK;
+  // what a launch gets unasked is 48 KB less the kernel's static shared memory (a few hundred bytes);
   // per device and kernel once would do; the call is cheap and has no state to go wrong
+  if (bytes <= 47 * 1024) return B200S_OK;
   B200S_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
   return B200S_OK;
 }

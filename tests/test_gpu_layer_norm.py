@@ -5,6 +5,10 @@ subnormal). Before that everything is fp32 with sums whose longest chain of addi
 c = d / 32 + 40 (a thread's share of the row, the warp's and the block's trees), each addition within
 2^-24 of the running value, so a mean carries c * 2^-24 of the mean absolute value.
 """
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -211,3 +215,32 @@ def test_long_batch_offsets_past_32_bits(b200s):
     dx, = torch.autograd.grad(y, x, g)
     check("last rows' dx", dx[-6:], want["dx"], torch.bfloat16)
     assert not dx[:-6].any()
+
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CHILD = r"""
+import sys, torch
+sys.path.insert(0, %r)
+import strassen_triton_b200 as b200s
+from tests.test_gpu_layer_norm import check, inputs, reference
+for rows, d, dtype in ((500, 3056, torch.bfloat16), (500, 3064, torch.float16), (700, 1528, torch.bfloat16),
+                       (700, 1744, torch.float16), (700, 1224, torch.float32)):
+    x, w, b, dy = inputs(rows, d, dtype, dtype)
+    want = reference(x, w, b, 1e-5, dy)
+    for t in (x, w, b):
+        t.requires_grad_(True)
+    y = b200s.layer_norm(x, w, b)
+    check("y", y.detach(), want["y"], dtype)
+    for name, got in zip(("dx", "dw", "db"), torch.autograd.grad(y, (x, w, b), dy)):
+        check(name, got, want[name], dtype)
+print("rows ok")
+""" % ROOT
+
+
+def test_row_lengths_whose_ring_just_fits_without_opting_in(built_library):
+    """Rings of 48 KB less a little: with the kernels' own shared memory they are above what a launch gets unasked. In a
+    process of its own, because a longer row before them raises the limit of the kernel they share."""
+    if not torch.cuda.is_available():
+        pytest.fail("this test needs a CUDA device")
+    out = subprocess.run([sys.executable, "-c", CHILD], cwd=ROOT, capture_output=True, text=True, timeout=600)
+    assert out.returncode == 0 and "rows ok" in out.stdout, out.stdout[-2000:] + out.stderr[-4000:]
