@@ -423,7 +423,7 @@ int b200s_epilogue_backward(int64_t M, int64_t N, int dtype, int activation, con
  *   y = act(x . weight^T + bias) + residual, z (the pre-activation) stored when given;
  *   dz = dy * act'(z), dx = dz . weight, dweight = dz^T . x, dbias = column sums of dz.
  * bias, residual, z may be NULL; so may dx, dweight and dbias, and z for B200S_ACT_NONE. Rows of any
- * length, alignment and stride are accepted: operands TMA cannot address are copied to scratch first.
+ * length (M, N, K up to 2^31 - 65537), alignment and stride are accepted: operands TMA cannot address are copied to scratch first.
  * M = 0 computes the gradients of an empty batch. Scratch, 256-byte aligned (NULL when the size is 0): the
  * matching _workspace bytes, with copies = 0 when every operand (x, weight; for the backward pass dy too) starts
  * on a 16-byte boundary and has rows a multiple of 16 bytes apart, else 1.

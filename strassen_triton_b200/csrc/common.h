@@ -91,6 +91,8 @@ struct LinearArgs {
   int64_t lda, ldb, ldc, ldr, ldz, ldp;
   int a_major, b_major, in_dtype, out_dtype, activation;
 };
+// Extents of the linear layer: coordinates of the last tile's far end must stay within 32 bits.
+constexpr int64_t kMaxLinearExtent = INT32_MAX - 65536;
 // How a product is computed, by its extents and majors alone.
 struct LinearPlan {
   enum Kind { kSkinny, kTiles } kind;

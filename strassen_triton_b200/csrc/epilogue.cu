@@ -417,7 +417,7 @@ static size_t product_scratch(int64_t M, int64_t N, int64_t K, int a_major, int 
 }
 
 static int check_linear(int64_t M, int64_t N, int64_t K, int dtype, int activation) {
-  if (M < 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) return B200S_ERR_BAD_SHAPE;
+  if (M < 0 || N <= 0 || K <= 0 || M > kMaxLinearExtent || N > kMaxLinearExtent || K > kMaxLinearExtent) return B200S_ERR_BAD_SHAPE;
   if (dtype != B200S_BF16 && dtype != B200S_FP16) return B200S_ERR_BAD_DTYPE;
   if (activation < B200S_ACT_NONE || activation > B200S_ACT_GELU_TANH) return B200S_ERR_BAD_ALGO;
   return B200S_OK;

@@ -697,7 +697,7 @@ LinearPlan plan_linear(int64_t M, int64_t N, int64_t K, int a_major, int b_major
 }
 
 int launch_linear(const LinearArgs& g, const LinearPlan& plan, cudaStream_t stream) {
-  if (g.M > INT32_MAX || g.N > INT32_MAX || g.K > INT32_MAX) return B200S_ERR_BAD_SHAPE;
+  if (g.M > kMaxLinearExtent || g.N > kMaxLinearExtent || g.K > kMaxLinearExtent) return B200S_ERR_BAD_SHAPE;
   if ((reinterpret_cast<uintptr_t>(g.A) & 15u) || (reinterpret_cast<uintptr_t>(g.B) & 15u)) return B200S_ERR_BAD_ALIGNMENT;
   if ((g.lda * 2) % 16 || (g.ldb * 2) % 16) return B200S_ERR_BAD_STRIDE;
   const bool bf16_out = g.out_dtype == B200S_BF16;

@@ -117,6 +117,18 @@ def test_linear_arguments(lib):
     assert back(dx=None, dw=None, db=None) == 0
 
 
+def test_linear_extents(lib):
+    """The far end of the last tile must have 32-bit coordinates: extents within 65536 of 2^31 are refused by both
+    ways to the kernels, before any of them runs."""
+    n = ctypes.c_size_t(0)
+    top = 2 ** 31 - 1 - 65536
+    for M, N, K in ((top + 1, 8, 8), (4, top + 1, 8), (4, 8, top + 1), (2 ** 31 - 1, 8, 8)):
+        assert lib.b200s_linear_act_workspace(M, N, K, _lib.BF16, 0, ctypes.byref(n)) == _lib.ERR_BAD_SHAPE
+        assert lib.b200s_linear_act_backward_workspace(M, N, K, _lib.BF16, _lib.ACT_NONE, 0, ctypes.byref(n)) == _lib.ERR_BAD_SHAPE
+        assert lib.b200s_linear_act(M, N, K, _lib.BF16, 0, 16, K, 16, K, None, None, 0, 16, N, None, 0, None, 0, None) == _lib.ERR_BAD_SHAPE
+    assert lib.b200s_linear_act_workspace(4, top, 8, _lib.BF16, 0, ctypes.byref(n)) == 0
+
+
 def test_logprob_arguments(lib):
     f = lib.b200s_token_logprobs
     args = dict(rows=4, vocab=8, dt=_lib.BF16, x=16, ld=8, t=16, ig=-100, lp=16, lse=16, ent=16, k=2, ids=16, top=16)
