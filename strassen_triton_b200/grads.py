@@ -84,10 +84,37 @@ def _sumsq(dev, arr, n, group):
     return total, 1
 
 
+def _no_share(device, group, error_if_nonfinite=False) -> Tensor:
+    """The norm on a rank that holds no gradient: it still takes its place in the sum over the ranks."""
+    import torch.distributed as dist
+
+    total = torch.zeros(1, dtype=torch.float64, device=device)
+    dist.all_reduce(total, group=group)
+    norm = total.sqrt().float().reshape(())
+    if error_if_nonfinite:
+        _require_finite(norm)
+    return norm
+
+
+def _require_finite(norm: Tensor) -> None:
+    if not math.isfinite(norm.item()):
+        raise RuntimeError("the norm of the gradients is not finite, so they cannot be clipped")
+
+
+def _bound(max_norm) -> float:
+    max_norm = float(max_norm)
+    if math.isnan(max_norm) or max_norm < 0:
+        raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
+    return max_norm
+
+
 def grad_norm(grads: Iterable[Tensor], *, group=None) -> Tensor:
     """sqrt of the sum of squares over all tensors, a 0-d float32 tensor, on the current stream. ``group``: a
-    process group whose ranks each hold a shard of the gradients; their sums of squares are added."""
+    process group whose ranks each hold a shard of the gradients; their sums of squares are added (a rank that
+    holds none passes an empty list)."""
     grads = list(grads)
+    if not grads and group is not None:
+        return _no_share(torch.device("cuda", torch.cuda.current_device()), group)
     words = _plain_words(grads)
     if words is not None:
         dev, arr = grads[0].device, array("q", words)
@@ -112,9 +139,9 @@ def clip_grads_(grads: Iterable[Tensor], max_norm: float, *, out: Optional[Seque
     makes all results NaN, unless ``error_if_nonfinite`` (which waits for the GPU) raises first. ``group`` as in
     `grad_norm`. A tensor that is written may appear only once and overlap no other one."""
     grads = list(grads)
-    max_norm = float(max_norm)
-    if math.isnan(max_norm) or max_norm < 0:
-        raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
+    max_norm = _bound(max_norm)
+    if not grads and group is not None:
+        return _no_share(torch.device("cuda", torch.cuda.current_device()), group, error_if_nonfinite)
     words = _plain_words(grads)
     dev = grads[0].device if words is not None else _checked(grads, "grads")
     src, back = grads, []
@@ -162,8 +189,7 @@ def clip_grads_(grads: Iterable[Tensor], max_norm: float, *, out: Optional[Seque
     norm = torch.empty((), dtype=torch.float32, device=dev)
     if error_if_nonfinite:
         call(dev, lib.b200s_grad_norm, parts.data_ptr(), n_parts, norm.data_ptr())
-        if not math.isfinite(norm.item()):
-            raise RuntimeError("the norm of the gradients is not finite, so they cannot be clipped")
+        _require_finite(norm)
     call(dev, lib.b200s_grad_clip, arr.buffer_info()[0], len(grads), parts.data_ptr(), n_parts, max_norm, norm.data_ptr())
     for t, s in back:
         t.copy_(s)
@@ -175,12 +201,17 @@ def clip_grads_(grads: Iterable[Tensor], max_norm: float, *, out: Optional[Seque
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, *,
                     group=None) -> Tensor:
     """torch.nn.utils.clip_grad_norm_ on the library's kernels: clips the ``grad`` of every parameter (those
-    without one are passed over) and returns the norm. Only the 2-norm is offered."""
+    without one are passed over) and returns the norm. Only the 2-norm is offered. ``group`` as in `grad_norm`; a
+    rank whose parameters have no gradients takes part in the sum."""
     if float(norm_type) != 2.0:
         raise ValueError(f"only norm_type 2 is offered, got {norm_type}")
     if isinstance(parameters, Tensor):
         parameters = [parameters]
+    parameters = list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
-        return torch.zeros(())
+        if group is None or not parameters:
+            return torch.zeros(())
+        _bound(max_norm)
+        return _no_share(parameters[0].device, group, error_if_nonfinite)
     return clip_grads_(grads, max_norm, error_if_nonfinite=error_if_nonfinite, group=group)

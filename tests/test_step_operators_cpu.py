@@ -194,6 +194,33 @@ def test_tensor_level_calls_refuse_cpu_tensors_and_bad_arguments():
         b200s.clip_grad_norm_([], 1.0, norm_type=1)
 
 
+def test_a_rank_without_gradients_takes_part_in_the_norm(monkeypatch):
+    """The other ranks wait in their all-reduce for it (a stand-in adds their squares here)."""
+    import torch.distributed as dist
+
+    import strassen_triton_b200 as b200s
+
+    calls = []
+
+    def all_reduce(t, group=None):
+        calls.append((group, t.dtype, t.tolist()))
+        t.add_(float(add))
+
+    monkeypatch.setattr(dist, "all_reduce", all_reduce)
+    params = [torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(2, 2))]
+    add = 9.0
+    n = b200s.clip_grad_norm_(params, 1.0, group="shards")
+    assert n.shape == () and n.dtype == torch.float32 and n.item() == 3.0
+    assert calls == [("shards", torch.float64, [0.0])]
+    assert b200s.clip_grad_norm_((p for p in params), 1.0).item() == 0.0 and len(calls) == 1
+    with pytest.raises(ValueError):
+        b200s.clip_grad_norm_(params, -1.0, group="shards")
+    assert len(calls) == 1
+    add = "nan"
+    with pytest.raises(RuntimeError, match="not finite"):
+        b200s.clip_grad_norm_(params, 1.0, error_if_nonfinite=True, group="shards")
+
+
 def test_dense_layouts():
     from strassen_triton_b200.grads import _dense
 
