@@ -42,6 +42,9 @@ def _checked(grads: Sequence[Tensor], what: str) -> torch.device:
             raise TypeError(f"unsupported dtype {t.dtype} in {what} (bfloat16, float16 and float32 are supported)")
         if t.layout is not torch.strided:
             raise TypeError(f"{what} must hold dense tensors")
+        if t.numel() and not t.data_ptr():
+            raise TypeError(f"{what} holds a {type(t).__name__} without memory of its own (of a sharded tensor pass the "
+                            "local part, and the process group)")
     return grads[0].device
 
 
@@ -56,8 +59,10 @@ def _plain_words(grads):
             if code is None or d < 0 or (d != dev and words) or t.layout is not torch.strided or not t.is_contiguous():
                 return None
             dev = d
-            p = t.data_ptr()
-            words += (p, p, t.numel(), code | code << 32)
+            p, n = t.data_ptr(), t.numel()
+            if not p and n:
+                return None
+            words += (p, p, n, code | code << 32)
     except AttributeError:
         return None
     return words or None

@@ -42,7 +42,8 @@ class LinearStrassen(nn.Linear):
         self.activation = activation
 
     def forward(self, input: Tensor, residual: Optional[Tensor] = None) -> Tensor:
-        """activation(input @ weight.T + bias) + residual; with no activation and no residual, the plain layer."""
+        """activation(input @ weight.T + bias) + residual; with no activation and no residual, the plain layer.
+        The residual (of the result's shape) is taken in the product's type: the weight's, autocast's under autocast."""
         *batch_dims, d_in = input.shape
         assert d_in == self.in_features, "Input dim mismatch"
         x = input.reshape(-1, d_in)
@@ -65,10 +66,11 @@ class LinearStrassen(nn.Linear):
             if depth == 0:
                 algo = "dense"
         if self.activation != "none" or residual is not None or self.one_call:
-            if residual is not None and residual.dtype != x.dtype:
-                residual = residual.to(x.dtype)
             if residual is not None:
-                residual = residual.reshape(-1, self.out_features)
+                if residual.shape != (*batch_dims, self.out_features):
+                    raise ValueError(f"residual must have the shape of the result {(*batch_dims, self.out_features)}, "
+                                     f"got {tuple(residual.shape)}")
+                residual = residual.to(x.dtype).reshape(-1, self.out_features)
             out = ops.linear_act(x, w, self.bias, self.activation, residual, algo=algo, depth=depth)
             return out.view(*batch_dims, self.out_features)
         # weight.T stays a view (model/layers.py:252); the bias rides in the product's epilogue

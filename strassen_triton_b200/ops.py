@@ -584,6 +584,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not form x @ weight.T")
     if algo not in _ALGO:
         raise ValueError(f"algo must be one of {sorted(_ALGO)}, got {algo!r}")
+    if precision is not None:
+        resolve_precision(precision)
     out_shape = x.shape[:-1] + (weight.shape[0],)
     if bias is not None:
         if bias.shape != out_shape[-1:]:

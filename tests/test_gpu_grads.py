@@ -238,3 +238,33 @@ def test_graph_and_repeats(b200s):
         t.mul_(2)
     g.replay()
     assert abs(n2.item() / norm64(grads) - 1) < 2.0 ** -22
+
+
+def test_tensors_without_memory_are_refused(b200s):
+    """A wrapper (a sharded tensor of torch's) has a device and a size, its memory is its local part's."""
+
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, t):
+            return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise AssertionError(f"{func} on a wrapper")
+
+    real = make([100], [torch.float32])[0]
+    for grads in ([Wrapper(real)], [real, Wrapper(real)]):
+        with pytest.raises(TypeError, match="Wrapper"):
+            b200s.grad_norm(grads)
+        with pytest.raises(TypeError, match="Wrapper"):
+            b200s.clip_grads_(grads, 1.0)
+
+
+def test_an_empty_list_with_a_group(b200s, monkeypatch):
+    import torch.distributed as dist
+
+    monkeypatch.setattr(dist, "all_reduce", lambda t, group=None: t.add_(16.0))
+    assert b200s.grad_norm([], group="shards").item() == 4.0
+    assert b200s.clip_grads_([], 1.0, group="shards").item() == 4.0
+    with pytest.raises(ValueError):
+        b200s.grad_norm([])

@@ -336,3 +336,11 @@ def test_linear_strassen_module(b200s):
     assert torch.equal(plain(x).view(100, 384), ops.matmul(x.view(100, 256), plain.weight.t(), algo="dense", bias=plain.bias))
     with pytest.raises(ValueError):
         LinearStrassen(8, 8, activation="tanh")
+
+
+def test_unknown_precision_is_refused_on_every_path(b200s):
+    for dtype in (torch.bfloat16, torch.float32):
+        x, w = torch.ones(4, 16, device="cuda", dtype=dtype), torch.ones(8, 16, device="cuda", dtype=dtype)
+        with pytest.raises(ValueError, match="precision"):
+            b200s.linear_act(x, w, precision="fp8")
+        assert torch.equal(b200s.linear_act(x, w, precision="tf32"), torch.full((4, 8), 16.0, device="cuda", dtype=dtype))

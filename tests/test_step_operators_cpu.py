@@ -221,6 +221,17 @@ def test_a_rank_without_gradients_takes_part_in_the_norm(monkeypatch):
         b200s.clip_grad_norm_(params, 1.0, error_if_nonfinite=True, group="shards")
 
 
+def test_residual_of_another_shape_is_refused():
+    """As many elements in other rows must not be added in silence."""
+    from strassen_triton_b200.linear import LinearStrassen
+
+    layer = LinearStrassen(8, 16, device="cpu", depth=0)
+    with pytest.raises(ValueError, match="residual"):
+        layer(torch.ones(2, 3, 8), residual=torch.ones(3, 2, 16))
+    with pytest.raises(ValueError, match="residual"):
+        layer(torch.ones(2, 3, 8), residual=torch.ones(6, 16))
+
+
 def test_dense_layouts():
     from strassen_triton_b200.grads import _dense
 
