@@ -89,25 +89,50 @@ __global__ void __launch_bounds__(kThreads) epilogue_kernel(const EpiloguePass p
   }
 }
 
-// Rows copied to where TMA can address them (a padded leading dimension; the padding is left alone).
+// Rows copied to where TMA can address them (a padded leading dimension; the padding is left alone), one or two
+// matrices by one launch.
+struct PadJob {
+  const uint16_t* in;
+  uint16_t* out;
+  int64_t rows, cols, ld_in, ld_out;
+  int blocks;      // of the launch that take this matrix's rows
+  int pairs;       // two elements an access
+};
+struct PadJobs {
+  PadJob job[2];
+  int count;
+};
 template <int VEC>
-__global__ void __launch_bounds__(kThreads) pad_rows_kernel(const uint16_t* in, uint16_t* out, int64_t rows, int64_t cols, int64_t ld_in,
-                                                            int64_t ld_out) {
+__device__ __forceinline__ void pad_rows(const PadJob& j, int64_t first) {
   using P = Pack<uint16_t, VEC>;
   constexpr int B = 4;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const uint16_t* from = in + r * ld_in;
-    uint16_t* to = out + r * ld_out;
+  const int64_t rows = j.rows, cols = j.cols, step = j.blocks;
+  for (int64_t r = first; r < rows; r += step) {
+    const uint16_t* from = j.in + r * j.ld_in;
+    uint16_t* to = j.out + r * j.ld_out;
     for (int64_t c0 = threadIdx.x * VEC; c0 < cols; c0 += B * kThreads * VEC) {
       P v[B];
 #pragma unroll
       for (int b = 0; b < B; ++b)
-        if (c0 + b * kThreads * VEC < cols) v[b] = row::ld<P>(from + c0 + b * kThreads * VEC);
+        if (c0 + b * kThreads * VEC < cols) v[b] = row::ld_const<P>(from + c0 + b * kThreads * VEC);
 #pragma unroll
       for (int b = 0; b < B; ++b)
         if (c0 + b * kThreads * VEC < cols) row::st(to + c0 + b * kThreads * VEC, v[b]);
     }
   }
+}
+__global__ void __launch_bounds__(kThreads) pad_rows_kernel(const __grid_constant__ PadJobs p) {
+  auto run = [](const PadJob& j, int64_t first) {
+    if (j.pairs)
+      pad_rows<2>(j, first);
+    else
+      pad_rows<1>(j, first);
+  };
+  const int block = static_cast<int>(blockIdx.x);
+  if (block < p.job[0].blocks)
+    run(p.job[0], block);
+  else
+    run(p.job[1], block - p.job[0].blocks);
 }
 
 struct EpilogueBwd {
@@ -427,26 +452,28 @@ static bool addressable(const void* p, int64_t ld, int64_t rows, int64_t cols) {
   return aligned(p, ld, rows, 2, 16) && (rows <= 1 || ld >= cols);
 }
 
-// `p`, or its rows copied to *scratch (which then moves on). *ld becomes the leading dimension to use.
-static int operand_rows(const void** p, int64_t* ld, int64_t rows, int64_t cols, uint8_t** scratch, cudaStream_t stream) {
+// `p`, or (by a job of *jobs) its rows copied to *scratch, which then moves on. *ld becomes the leading dimension
+// to use.
+static void operand_rows(const void** p, int64_t* ld, int64_t rows, int64_t cols, uint8_t** scratch, PadJobs* jobs) {
   if (addressable(*p, *ld, rows, cols)) {
     if (rows <= 1) *ld = padded(cols);
-    return B200S_OK;
+    return;
   }
-  const uint16_t* in = static_cast<const uint16_t*>(*p);
-  uint16_t* out = reinterpret_cast<uint16_t*>(*scratch);
-  const int64_t to = padded(cols);
-  const bool pairs = cols % 2 == 0 && aligned(in, *ld, rows, 2, 4);
-  const unsigned grid = static_cast<unsigned>(rows < 148 * 16 ? rows : 148 * 16);
-  if (pairs)
-    pad_rows_kernel<2><<<grid, kThreads, 0, stream>>>(in, out, rows, cols, *ld, to);
-  else
-    pad_rows_kernel<1><<<grid, kThreads, 0, stream>>>(in, out, rows, cols, *ld, to);
+  PadJob& j = jobs->job[jobs->count++];
+  j.in = static_cast<const uint16_t*>(*p);
+  j.out = reinterpret_cast<uint16_t*>(*scratch);
+  j.rows = rows, j.cols = cols, j.ld_in = *ld, j.ld_out = padded(cols);
+  j.blocks = static_cast<int>(rows < 148 * 16 ? rows : 148 * 16);
+  j.pairs = cols % 2 == 0 && aligned(j.in, *ld, rows, 2, 4);
+  *p = j.out;
+  *ld = j.ld_out;
+  *scratch += rows_bytes(rows, cols);
+}
+static int run_jobs(const PadJobs& jobs, cudaStream_t stream) {
+  if (jobs.count == 0) return B200S_OK;
+  pad_rows_kernel<<<static_cast<unsigned>(jobs.job[0].blocks + (jobs.count > 1 ? jobs.job[1].blocks : 0)), kThreads, 0, stream>>>(jobs);
   B200S_CUDA_OK(cudaGetLastError());
   count_launch();
-  *p = out;
-  *ld = to;
-  *scratch += rows_bytes(rows, cols);
   return B200S_OK;
 }
 
@@ -488,8 +515,10 @@ int b200s_linear_act(int64_t M, int64_t N, int64_t K, int dtype, int activation,
   if (!device_status_words()) return B200S_ERR_NO_DEVICE;
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   uint8_t* scratch = static_cast<uint8_t*>(workspace);
-  if ((rc = operand_rows(&x, &ldx, M, K, &scratch, stream)) != 0) return rc;
-  if ((rc = operand_rows(&weight, &ldw, N, K, &scratch, stream)) != 0) return rc;
+  PadJobs jobs = {};
+  operand_rows(&x, &ldx, M, K, &scratch, &jobs);
+  operand_rows(&weight, &ldw, N, K, &scratch, &jobs);
+  if ((rc = run_jobs(jobs, stream)) != 0) return rc;
   const LinearArgs g{x, weight, y, bias, residual, z, nullptr, M, N, K, ldx, ldw, ldy, ldr, ldz, 0, B200S_K_MAJOR, B200S_K_MAJOR, dtype, dtype, activation};
   return run_linear(g, scratch, stream);
 }
@@ -555,12 +584,10 @@ int b200s_linear_act_backward(int64_t M, int64_t N, int64_t K, int dtype, int ac
     rc = b200s_epilogue_backward(M, N, dtype, activation, z, ldz, dy, lddy, own ? const_cast<void*>(dz) : nullptr, lddz, dbias, parts, sums, stream_v);
     if (rc) return rc;
   }
-  if (dx) {
-    if ((rc = operand_rows(&weight, &ldw, N, K, &scratch, stream)) != 0) return rc;
-  }
-  if (dweight) {
-    if ((rc = operand_rows(&x, &ldx, M, K, &scratch, stream)) != 0) return rc;
-  }
+  PadJobs jobs = {};
+  if (dx) operand_rows(&weight, &ldw, N, K, &scratch, &jobs);
+  if (dweight) operand_rows(&x, &ldx, M, K, &scratch, &jobs);
+  if ((rc = run_jobs(jobs, stream)) != 0) return rc;
   if (dx) {
     const LinearArgs g{dz, weight, dx, nullptr, nullptr, nullptr, nullptr, M, K, N, lddz, ldw, lddx, 0, 0, 0, B200S_K_MAJOR, B200S_MN_MAJOR, dtype, dtype, B200S_ACT_NONE};
     if ((rc = run_linear(g, scratch, stream)) != 0) return rc;
