@@ -43,10 +43,24 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def empty(n: int, dtype, device) -> torch.Tensor:
+    """torch.empty(n) (an allocation with its strides given costs 1.5 us, one without 2.3)."""
+    return torch.empty_strided((n,), (1,), dtype=dtype, device=device)
+
+
+def empty_rows(rows: int, cols: int, dtype, device) -> torch.Tensor:
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
+def empty_as(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def call(device: torch.device, fn, *args) -> None:
     """fn(*args, stream) on the current stream of ``device``; a negative status raises."""
     index = device.index
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -79,4 +93,8 @@ def once(backward):
 
 
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False

@@ -15,7 +15,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._call import DTYPE, call, require_cuda
+from ._call import DTYPE, call, empty, require_cuda
 
 
 def _dense(t: Tensor) -> bool:
@@ -91,7 +91,7 @@ def _entries(src, dst):
 
 def _sumsq(dev, arr, n, group):
     """(parts, how many of them count): the partial sums of squares, of all ranks of ``group`` when given."""
-    parts = torch.empty(_lib.NORM_PARTS, dtype=torch.float64, device=dev)
+    parts = empty(_lib.NORM_PARTS, torch.float64, dev)
     call(dev, _lib.load().b200s_grad_sumsq, arr.buffer_info()[0], n, parts.data_ptr())
     if group is None:
         return parts, _lib.NORM_PARTS
@@ -141,7 +141,7 @@ def grad_norm(grads: Iterable[Tensor], *, group=None) -> Tensor:
         grads = [t if _dense(t) else t.contiguous() for t in grads]
         arr = _entries(grads, grads)
     parts, n_parts = _sumsq(dev, arr, len(grads), group)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
+    norm = torch.empty_strided((), (), dtype=torch.float32, device=dev)
     call(dev, _lib.load().b200s_grad_norm, parts.data_ptr(), n_parts, norm.data_ptr())
     return norm
 
@@ -204,7 +204,7 @@ def clip_grads_(grads: Iterable[Tensor], max_norm: float, *, out: Optional[Seque
             arr = _entries(src, dst)
     lib = _lib.load()
     parts, n_parts = _sumsq(dev, arr, len(grads), group)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
+    norm = torch.empty_strided((), (), dtype=torch.float32, device=dev)
     if error_if_nonfinite:
         call(dev, lib.b200s_grad_norm, parts.data_ptr(), n_parts, norm.data_ptr())
         _require_finite(norm)

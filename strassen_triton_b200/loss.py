@@ -14,7 +14,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._call import call, dtype_code, once, ptr, require_cuda, rows_of, wants_grad
+from ._call import call, dtype_code, empty_as, once, ptr, require_cuda, rows_of, wants_grad
 
 
 class TokenLogprobs(NamedTuple):
@@ -26,14 +26,13 @@ class TokenLogprobs(NamedTuple):
 
 def _forward(logits, targets, vocab, ignore_index, entropy, top_k, lse):
     xr, rows, ld = rows_of(logits)
-    shape, dev = targets.shape, logits.device
     t = targets.contiguous()
-    lp = torch.empty(shape, dtype=torch.float32, device=dev)
-    ent = torch.empty(shape, dtype=torch.float32, device=dev) if entropy else None
-    ls = torch.empty(shape, dtype=torch.float32, device=dev) if lse else None
-    ids = torch.empty(shape + (top_k,), dtype=torch.int64, device=dev) if top_k else None
-    top = torch.empty(shape + (top_k,), dtype=torch.float32, device=dev) if top_k else None
-    call(dev, _lib.load().b200s_token_logprobs, rows, vocab, dtype_code(logits, "logits"), xr.data_ptr(), ld, t.data_ptr(),
+    lp = torch.empty_like(t, dtype=torch.float32)
+    ent = torch.empty_like(lp) if entropy else None
+    ls = torch.empty_like(lp) if lse else None
+    ids = t.new_empty(t.shape + (top_k,)) if top_k else None
+    top = torch.empty_like(ids, dtype=torch.float32) if top_k else None
+    call(logits.device, _lib.load().b200s_token_logprobs, rows, vocab, dtype_code(logits, "logits"), xr.data_ptr(), ld, t.data_ptr(),
          ignore_index, lp.data_ptr(), ptr(ls), ptr(ent), top_k, ptr(ids), ptr(top))
     return lp, ls, ent, ids, top
 
@@ -43,7 +42,7 @@ def _backward(logits, targets, vocab, ignore_index, lse, entropy, dlogprob, dent
     t = targets.contiguous()
     dl, de = (g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.to(torch.float32).contiguous()
               for g in (dlogprob, dentropy))
-    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    out = empty_as(logits)
     width = logits.shape[-1]
     call(logits.device, _lib.load().b200s_token_logprobs_backward, rows, vocab, width, dtype_code(logits, "logits"),
          xr.data_ptr(), ld, t.data_ptr(), ignore_index, lse.data_ptr(), ptr(entropy if de is not None else None),

@@ -16,7 +16,7 @@ import torch.nn as nn
 from torch import Tensor
 
 from . import _lib
-from ._call import DTYPE, call, dtype_code, once, ptr, require_cuda, rows_of, wants_grad
+from ._call import DTYPE, call, dtype_code, empty, empty_as, empty_rows, once, ptr, require_cuda, rows_of, wants_grad
 
 
 def _check(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]) -> None:
@@ -43,13 +43,13 @@ def _dense(p):
 def _forward(x, weight, bias, eps, stats):
     """(y, statistics): two rows of fp32 values, mean and rstd, or None without ``stats``."""
     xr, rows, ldx = rows_of(x)
-    y = torch.empty_like(x) if xr is x and x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = empty_as(x)
     w, b = _dense(weight), _dense(bias)
     d = x.shape[-1]
     p = w if w is not None else b
     st, mean, rstd = None, None, None
     if stats:
-        st = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        st = empty_rows(2, rows, torch.float32, x.device)
         mean = st.data_ptr()
         rstd = mean + 4 * rows
         if rows == 0:
@@ -75,13 +75,13 @@ def _backward(dy, x, weight, st, param_dtype, need_x, need_w, need_b):
     gr, _, ldg = rows_of(dy)
     d, dev = x.shape[-1], x.device
     w = _dense(weight)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-    dw = torch.empty(d, dtype=param_dtype, device=dev) if need_w else None
-    db = torch.empty(d, dtype=param_dtype, device=dev) if need_b else None
+    dx = empty_as(x) if need_x else None
+    dw = empty(d, param_dtype, dev) if need_w else None
+    db = empty(d, param_dtype, dev) if need_b else None
     ws, need = None, 0
     if need_w or need_b:
         need = _workspace_bytes(rows, d)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)     # held until the launch
+        ws = empty(need, torch.uint8, dev)     # held until the launch
     mean = st.data_ptr()
     call(dev, _lib.load().b200s_layer_norm_backward, rows, d, DTYPE[x.dtype], DTYPE[param_dtype], xr.data_ptr(), ldx,
          gr.data_ptr(), ldg, ptr(w), mean, mean + 4 * rows, ptr(dx), d, ptr(dw), ptr(db), ptr(ws), need)

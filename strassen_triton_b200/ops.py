@@ -431,11 +431,11 @@ def _dense_forward(x, weight, bias, residual, act, save):
     """(y, z): z has its rows padded to whole 16-byte vectors, None when the backward pass needs none."""
     M, K = x.shape
     N, dt, dev = weight.shape[0], x.dtype, x.device
-    y = torch.empty((M, N), dtype=dt, device=dev)
+    y = _call.empty_rows(M, N, dt, dev)
     z, ldz = None, 0
     if save and act:
         ldz = (N + 7) // 8 * 8
-        z = torch.empty((M, ldz), dtype=dt, device=dev)
+        z = _call.empty_rows(M, ldz, dt, dev)
     rp, ldr = None, 0
     if residual is not None:
         if not _rows_contiguous(residual):
@@ -444,7 +444,7 @@ def _dense_forward(x, weight, bias, residual, act, save):
     code = _DTYPE[dt]
     need = _dense_workspace(False, M, N, K, code, 0, 1 if _off_grid(x) or _off_grid(weight) else 0)
     # held until the launch: freed, it could go to another thread's call on this stream before that
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = _call.empty(need, torch.uint8, dev) if need else None
     _call.call(dev, _lib.load().b200s_linear_act, M, N, K, code, act, x.data_ptr(), x.stride(0), weight.data_ptr(),
                weight.stride(0), None if bias is None else bias.data_ptr(), rp, ldr, y.data_ptr(), N,
                None if z is None else z.data_ptr(), ldz, None if ws is None else ws.data_ptr(), need)
@@ -458,12 +458,12 @@ def _dense_backward(dy, x, weight, z, act, need_x, need_w, need_b):
         dy = dy.to(dt)
     if not _rows_contiguous(dy):
         dy = dy.contiguous()
-    dx = torch.empty((M, K), dtype=dt, device=dev) if need_x else None
-    dw = torch.empty((N, K), dtype=dt, device=dev) if need_w else None
-    db = torch.empty(N, dtype=dt, device=dev) if need_b else None
+    dx = _call.empty_rows(M, K, dt, dev) if need_x else None
+    dw = _call.empty_rows(N, K, dt, dev) if need_w else None
+    db = _call.empty(N, dt, dev) if need_b else None
     code = _DTYPE[dt]
     need = _dense_workspace(True, M, N, K, code, act, 1 if _off_grid(x) or _off_grid(weight) or _off_grid(dy) else 0)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = _call.empty(need, torch.uint8, dev)
     p = _call.ptr
     _call.call(dev, _lib.load().b200s_linear_act_backward, M, N, K, code, act, x.data_ptr(), x.stride(0), weight.data_ptr(),
                weight.stride(0), p(z), z.shape[1] if z is not None else 0, dy.data_ptr(), dy.stride(0), p(dx), K, p(dw), K,
