@@ -146,11 +146,12 @@ struct EpilogueBwd {
 
 // 32 VEC columns per block, 8 rows at a time; a slice takes rows slice * 8 + warp, + slices * 8, ... Columns stay
 // with their thread, so the sums of dz add up in registers, unrounded. Reads z and dy, writes dz: 8192 x 2304 bf16
-// with GELU takes 26 us (113 MB, 4.3 TB/s; the two special functions and 20 instructions a pair weigh as much).
+// with GELU takes 25 us (113 MB, 4.5 TB/s; the two special functions and 20 instructions a pair weigh as much).
+// (Two rows on their way and four blocks an SM; four rows and three blocks 26, two and six, with spills, 30.)
 template <typename T, int ACT, int VEC>
-__global__ void __launch_bounds__(kThreads) epilogue_bwd_kernel(const EpilogueBwd p) {
+__global__ void __launch_bounds__(kThreads, 4) epilogue_bwd_kernel(const EpilogueBwd p) {
   using P = Pack<T, VEC>;
-  constexpr int R = 4;      // rows on their way per thread
+  constexpr int R = 2;      // rows on their way per thread
   __shared__ float sb[8][32 * VEC + 1];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + tx) * VEC;
