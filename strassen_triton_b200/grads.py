@@ -220,7 +220,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
                     group=None) -> Tensor:
     """torch.nn.utils.clip_grad_norm_ on the library's kernels: clips the ``grad`` of every parameter (those
     without one are passed over) and returns the norm. Only the 2-norm is offered. ``group`` as in `grad_norm`; a
-    rank whose parameters have no gradients takes part in the sum."""
+    rank that has no parameters, or none with a gradient, takes part in the sum."""
     if float(norm_type) != 2.0:
         raise ValueError(f"only norm_type 2 is offered, got {norm_type}")
     if isinstance(parameters, Tensor):
@@ -228,8 +228,9 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     parameters = list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
-        if group is None or not parameters:
+        if group is None:
             return torch.zeros(())
         _bound(max_norm)
-        return _no_share(parameters[0].device, group, error_if_nonfinite)
+        device = parameters[0].device if parameters else torch.device("cuda", torch.cuda.current_device())
+        return _no_share(device, group, error_if_nonfinite)
     return clip_grads_(grads, max_norm, error_if_nonfinite=error_if_nonfinite, group=group)
