@@ -465,6 +465,22 @@ int b200s_token_logprobs_backward(int64_t rows, int64_t vocab, int64_t width, in
                                   const float* lse_device, const float* entropy_device, const float* dlogprob_device,
                                   const float* dentropy_device, void* dlogits_device, int64_t ldd, void* stream);
 
+/*
+ * The same pair with each row's statistics in two parts: `stats` (8-byte aligned, may be NULL in the forward
+ * call) holds the largest logit and the log of the sum of e^(logit - largest), two fp32 values a row. Their sum
+ * is lse, but as one fp32 value lse is good to |lse| 2^-24 only and every probability the backward pass forms
+ * from it carries that: with logits around 1e4 the gradients above are good to 5e-4, these to a few 1e-6.
+ */
+int b200s_token_logprobs_stats(int64_t rows, int64_t vocab, int dtype, const void* logits_device, int64_t ld,
+                               const int64_t* targets_device, int64_t ignore_index, float* logprob_device,
+                               float* stats_device, float* entropy_device, int top_k, int64_t* top_ids_device,
+                               float* top_logprobs_device, void* stream);
+int b200s_token_logprobs_backward_stats(int64_t rows, int64_t vocab, int64_t width, int dtype, const void* logits_device,
+                                        int64_t ld, const int64_t* targets_device, int64_t ignore_index,
+                                        const float* stats_device, const float* entropy_device,
+                                        const float* dlogprob_device, const float* dentropy_device, void* dlogits_device,
+                                        int64_t ldd, void* stream);
+
 /* One dense tensor of a list: numel elements at src; dst, where a call writes, may be src itself. */
 typedef struct b200s_tensor {
   const void* src;

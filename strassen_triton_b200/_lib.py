@@ -148,6 +148,9 @@ SIGNATURES = {
     "b200s_token_logprobs": (_INT, [_I64, _I64, _INT, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _INT, _PTR, _PTR, _PTR]),
     "b200s_token_logprobs_backward": (_INT, [_I64, _I64, _I64, _INT, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _PTR, _PTR,
                                              _I64, _PTR]),
+    "b200s_token_logprobs_stats": (_INT, [_I64, _I64, _INT, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _INT, _PTR, _PTR, _PTR]),
+    "b200s_token_logprobs_backward_stats": (_INT, [_I64, _I64, _I64, _INT, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _PTR, _PTR,
+                                                   _I64, _PTR]),
     "b200s_grad_sumsq": (_INT, [_PTR, _I64, _PTR, _PTR]),
     "b200s_grad_norm": (_INT, [_PTR, _INT, _PTR, _PTR]),
     "b200s_grad_clip": (_INT, [_PTR, _I64, _PTR, _INT, _F32, _PTR, _PTR]),

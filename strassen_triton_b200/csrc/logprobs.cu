@@ -3,9 +3,11 @@
 //
 //   m = max x, s = sum e^(x-m), u = sum e^(x-m) (x-m)      one pass, m running
 //   lse = m + log s, logprob = x_t - lse, entropy = log s - u / s
-//   dx_i = gl (1[i = t] - p_i) - ge p_i (log p_i + entropy),  p_i = e^(x_i - lse)
+//   dx_i = gl (1[i = t] - p_i) - ge p_i (log p_i + entropy),  p_i = e^(x_i - m) / s
 //
-// The running maximum, both sums and everything derived from them are fp32. A forbidden token (-inf)
+// The running maximum, both sums and everything derived from them are fp32. The backward pass takes m and log s
+// apart: their sum lse is good to |lse| 2^-24 only, which every probability formed from it would carry (logits
+// around 1e4: 5e-4 of p; from the two parts a few 1e-6 wherever the logits lie). A forbidden token (-inf)
 // has probability zero and takes no part in u. A row without any finite logit has no distribution:
 // its logprob and lse are -inf, its entropy and its gradient zero. NaN (or +inf) among the logits
 // makes the row's results NaN. A target equal to ignore_index gives logprob 0 and no gradient from
@@ -117,13 +119,14 @@ struct LogprobFwd {
   const void* logits;
   const int64_t* targets;
   float* logprob;
-  float* lse;
+  float* stats;        // of every row lse, or its two parts: maximum and log of the sum; may be null
   float* entropy;
   int64_t* top_ids;
   float* top_logprobs;
   int64_t rows, ld, ignore_index;
   int32_t vocab, top_k;
   int32_t parts;       // CTAs (a cluster) that share a row
+  int32_t split_stats;
 };
 
 // The elements of a row as a head up to the first 16-byte boundary, a body of 16-byte vectors and a tail.
@@ -429,7 +432,12 @@ __global__ void __launch_bounds__(kThreads, 5) logprob_fwd_kernel(const LogprobF
           lp = lse == kNegInf ? kNegInf : (to_f(x[t]) - a.m) - logs;
         }
         p.logprob[r] = lp;
-        if (p.lse) p.lse[r] = lse;
+        if (p.stats) {
+          if (p.split_stats)
+            reinterpret_cast<float2*>(p.stats)[r] = make_float2(a.m, logs);
+          else
+            p.stats[r] = lse;
+        }
         if (ENT) p.entropy[r] = lse == kNegInf ? 0.f : logs - a.u / a.s;
         row_result = make_float2(lse == kNegInf ? kNegInf : a.m, logs);
       }
@@ -461,7 +469,8 @@ __global__ void __launch_bounds__(kThreads, 5) logprob_fwd_kernel(const LogprobF
 struct LogprobBwd {
   const void* logits;
   const int64_t* targets;
-  const float* lse;
+  const float2* stats;     // maximum and log of the sum, or null:
+  const float* lse;        // their sum instead
   const float* entropy;
   const float* dlogprob;   // may be null
   const float* dentropy;   // may be null
@@ -472,6 +481,9 @@ struct LogprobBwd {
 
 // One row per block of the grid's first dimension (the last rows first: the forward pass left their logits in
 // L2), its vectors dealt to the blocks of the second.
+// Few values live through the loop, so that 32 registers do and eight blocks are resident (8192 x 50304 bf16: 251 us,
+// with one register more 272; with an entropy's gradient 270 instead of 301): both gradients are taken times 1 / s,
+// and the thread that has the target's column writes it once more at the end.
 template <typename T, bool ENT>
 __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobBwd p) {
   constexpr int V = 16 / sizeof(T);
@@ -480,38 +492,40 @@ __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobBwd 
   const T* x = static_cast<const T*>(p.logits) + r * p.ld;
   T* d = static_cast<T*>(p.dlogits) + r * p.ldd;
   const int64_t t = p.targets[r];
-  const float lse = p.lse[r];
+  const float2 st = p.stats ? p.stats[r] : make_float2(p.lse[r], 0.f);
+  const float m = st.x, lse = st.x + st.y;
   const bool ignored = t == p.ignore_index;
   float gl = p.dlogprob && !ignored ? p.dlogprob[r] : 0.f;
-  const float ge = ENT ? p.dentropy[r] : 0.f;
-  const float h = ENT ? p.entropy[r] : 0.f;
+  float ge = ENT ? p.dentropy[r] : 0.f;
+  const float h = ENT ? p.entropy[r] - st.y : 0.f;      // log p_i + entropy = (x_i - m) + h
   if (!ignored && (t < 0 || t >= p.vocab)) gl = nan_f();
-  const int target = t >= 0 && t < p.vocab && !ignored ? static_cast<int>(t) : -1;
   // an ignored row stays zero whatever its logits hold
   const bool none = lse == kNegInf || (gl == 0.f && ge == 0.f && (ignored || lse == lse));
   const int limit = none ? 0 : p.vocab;
-  auto one = [&](int c) {
-    float v = 0.f;
-    if (c < limit) {
-      const float lp = to_f(x[c]) - lse;
-      const float pr = exp2_approx(lp * kLog2e);
-      v = -gl * pr;
-      if constexpr (ENT) v -= ge * pr * (fmaxf(lp, -1000.f) + h);
-      if (c == target) v += gl;
-    }
-    d[c] = from_f<T>(v);
+  const int target = t >= 0 && t < limit && !ignored ? static_cast<int>(t) : -1;
+  const float gt = gl;
+  gl *= expf(-st.y);
+  if constexpr (ENT) ge *= expf(-st.y);
+  auto value = [&](float x, float own) {
+    const float gap = x - m;
+    const float e = exp2_approx(gap * kLog2e);
+    float v = fmaf(-gl, e, own);
+    if constexpr (ENT) v -= ge * e * (fmaxf(gap, -1000.f) + h);
+    return v;
   };
+  auto one = [&](int c, float own) { d[c] = from_f<T>(c < limit ? value(to_f(x[c]), own) : 0.f); };
   const int first = static_cast<int>(blockIdx.y) * kThreads + static_cast<int>(threadIdx.x);
   const int step = static_cast<int>(gridDim.y) * kThreads;
   const bool paired = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15u) == 0;
   if (!paired) {
-    for (int c = first; c < p.width; c += step) one(c);
+    for (int c = first; c < p.width; c += step) one(c, c == target ? gt : 0.f);
     return;
   }
   const RowSpan<T> sp(d, p.width);
-  if (first < sp.head) one(first);
-  if (sp.tail() + first < p.width) one(sp.tail() + first);
-  const float2 sh = make_float2(-lse, -lse), l2 = make_float2(kLog2e, kLog2e), ng = make_float2(-gl, -gl);
+  if (first < sp.head) one(first, first == target ? gt : 0.f);
+  if (sp.tail() + first < p.width) one(sp.tail() + first, sp.tail() + first == target ? gt : 0.f);
+  const T at_target = x[target >= 0 ? target : 0];      // before its vector is written: d may be x
+  const float2 sh = make_float2(-m, -m), l2 = make_float2(kLog2e, kLog2e), ng = make_float2(-gl, -gl);
   const float2 ne = make_float2(-ge, -ge), hh = make_float2(h, h);
 #pragma unroll 4
   for (int i = first; i < sp.vecs; i += step) {
@@ -521,22 +535,12 @@ __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobBwd 
       const P v = row::ld<P>(x + c);
 #pragma unroll
       for (int k = 0; k < V / 2; ++k) {
-        const float2 lp = row::add_(row::load2(v.e + 2 * k), sh);
-        const float2 q = row::mul_(lp, l2);
-        const float2 pr = make_float2(exp2_approx(q.x), exp2_approx(q.y));
+        const float2 gap = row::add_(row::load2(v.e + 2 * k), sh);
+        const float2 q = row::mul_(gap, l2);
+        const float2 e = make_float2(exp2_approx(q.x), exp2_approx(q.y));
         float2 g = ng;
-        if constexpr (ENT) g = row::fma_(ne, row::add_(make_float2(fmaxf(lp.x, -1000.f), fmaxf(lp.y, -1000.f)), hh), g);
-        row::store2(out.e + 2 * k, row::mul_(g, pr));
-      }
-      if (static_cast<unsigned>(target - c) < static_cast<unsigned>(V)) {
-        // the target's own column, from fp32 again
-        const float lp = to_f(x[target]) - lse;
-        const float pr = exp2_approx(lp * kLog2e);
-        float w = fmaf(-gl, pr, gl);
-        if constexpr (ENT) w -= ge * pr * (fmaxf(lp, -1000.f) + h);
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (c + e == target) out.e[e] = from_f<T>(w);
+        if constexpr (ENT) g = row::fma_(ne, row::add_(make_float2(fmaxf(gap.x, -1000.f), fmaxf(gap.y, -1000.f)), hh), g);
+        row::store2(out.e + 2 * k, row::mul_(g, e));
       }
       row::st(d + c, out);
     } else if (c >= limit) {
@@ -544,9 +548,11 @@ __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobBwd 
       for (int e = 0; e < V; ++e) out.e[e] = from_f<T>(0.f);
       row::st(d + c, out);
     } else {
-      for (int e = 0; e < V; ++e) one(c + e);
+      for (int e = 0; e < V; ++e) one(c + e, 0.f);
     }
   }
+  const int at = target - sp.head;
+  if (at >= 0 && target < sp.tail() && (at / V - first) % step == 0) d[target] = from_f<T>(value(to_f(at_target), p.dlogprob ? p.dlogprob[r] : 0.f));
 }
 
 int check_logits(int64_t rows, int64_t vocab, int dtype) {
@@ -602,7 +608,9 @@ int launch_bwd(const LogprobBwd& p, cudaStream_t stream) {
     q.rows = n;
     q.logits = static_cast<const T*>(p.logits) + r0 * p.ld;
     q.dlogits = static_cast<T*>(p.dlogits) + r0 * p.ldd;
-    q.targets = p.targets + r0, q.lse = p.lse + r0;
+    q.targets = p.targets + r0;
+    if (p.stats) q.stats = p.stats + r0;
+    if (p.lse) q.lse = p.lse + r0;
     if (p.entropy) q.entropy = p.entropy + r0;
     if (p.dlogprob) q.dlogprob = p.dlogprob + r0;
     if (p.dentropy) q.dentropy = p.dentropy + r0;
@@ -623,11 +631,10 @@ int launch_bwd(const LogprobBwd& p, cudaStream_t stream) {
 
 using namespace b200s;
 
-extern "C" {
-
-int b200s_token_logprobs(int64_t rows, int64_t vocab, int dtype, const void* logits, int64_t ld, const int64_t* targets,
-                         int64_t ignore_index, float* logprob, float* lse, float* entropy, int top_k, int64_t* top_ids,
-                         float* top_logprobs, void* stream) {
+// Both forward entries: lse, or stats (a maximum and a log of the sum per row), or neither.
+static int logprobs_forward(int64_t rows, int64_t vocab, int dtype, const void* logits, int64_t ld, const int64_t* targets,
+                            int64_t ignore_index, float* logprob, float* lse, float* stats, float* entropy, int top_k,
+                            int64_t* top_ids, float* top_logprobs, void* stream) {
   int rc = check_logits(rows, vocab, dtype);
   if (rc) return rc;
   if (top_k < 0 || top_k > kMaxTopK || top_k > vocab) return B200S_ERR_BAD_SHAPE;
@@ -636,37 +643,70 @@ int b200s_token_logprobs(int64_t rows, int64_t vocab, int dtype, const void* log
   if (top_k > 0 && (!top_ids || !top_logprobs)) return B200S_ERR_NULL_POINTER;
   if (rows > 1 && ld < 0) return B200S_ERR_BAD_STRIDE;
   if (misaligned(logits, dtype_size(dtype)) || misaligned(targets, 8) || misaligned(logprob, 4) || misaligned(lse, 4) ||
-      misaligned(entropy, 4) || misaligned(top_ids, 8) || misaligned(top_logprobs, 4))
+      misaligned(stats, 8) || misaligned(entropy, 4) || misaligned(top_ids, 8) || misaligned(top_logprobs, 4))
     return B200S_ERR_BAD_ALIGNMENT;
   if (!device_status_words()) return B200S_ERR_NO_DEVICE;
-  const LogprobFwd p{logits, targets, logprob, lse, entropy, top_ids, top_logprobs, rows, ld, ignore_index,
-                     static_cast<int32_t>(vocab), top_k, row_parts(rows, vocab)};
+  const LogprobFwd p{logits, targets, logprob, stats ? stats : lse, entropy, top_ids, top_logprobs, rows, ld, ignore_index,
+                     static_cast<int32_t>(vocab), top_k, row_parts(rows, vocab), stats ? 1 : 0};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == B200S_BF16) return launch_fwd<__nv_bfloat16>(p, s);
   if (dtype == B200S_FP16) return launch_fwd<__half>(p, s);
   return launch_fwd<float>(p, s);
 }
 
-int b200s_token_logprobs_backward(int64_t rows, int64_t vocab, int64_t width, int dtype, const void* logits, int64_t ld,
-                                  const int64_t* targets, int64_t ignore_index, const float* lse, const float* entropy,
-                                  const float* dlogprob, const float* dentropy, void* dlogits, int64_t ldd,
-                                  void* stream) {
+// Both backward entries: one of lse and stats.
+static int logprobs_backward(int64_t rows, int64_t vocab, int64_t width, int dtype, const void* logits, int64_t ld,
+                             const int64_t* targets, int64_t ignore_index, const float* lse, const float* stats,
+                             const float* entropy, const float* dlogprob, const float* dentropy, void* dlogits, int64_t ldd,
+                             void* stream) {
   int rc = check_logits(rows, vocab, dtype);
   if (rc) return rc;
   if (width < vocab || width > INT32_MAX - 65536) return B200S_ERR_BAD_SHAPE;
   if (rows == 0) return B200S_OK;
-  if (!logits || !targets || !lse || !dlogits || (dentropy && !entropy)) return B200S_ERR_NULL_POINTER;
+  if (!logits || !targets || (!lse && !stats) || !dlogits || (dentropy && !entropy)) return B200S_ERR_NULL_POINTER;
   if (rows > 1 && (ld < 0 || ldd < width)) return B200S_ERR_BAD_STRIDE;
   if (misaligned(logits, dtype_size(dtype)) || misaligned(dlogits, dtype_size(dtype)) || misaligned(targets, 8) ||
-      misaligned(lse, 4) || misaligned(entropy, 4) || misaligned(dlogprob, 4) || misaligned(dentropy, 4))
+      misaligned(lse, 4) || misaligned(stats, 8) || misaligned(entropy, 4) || misaligned(dlogprob, 4) || misaligned(dentropy, 4))
     return B200S_ERR_BAD_ALIGNMENT;
   if (!device_status_words()) return B200S_ERR_NO_DEVICE;
-  const LogprobBwd p{logits, targets, lse, entropy, dlogprob, dentropy, dlogits, rows, ld, ldd, ignore_index,
-                     static_cast<int32_t>(vocab), static_cast<int32_t>(width)};
+  const LogprobBwd p{logits, targets, reinterpret_cast<const float2*>(stats), lse, entropy, dlogprob, dentropy, dlogits, rows, ld,
+                     ldd, ignore_index, static_cast<int32_t>(vocab), static_cast<int32_t>(width)};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == B200S_BF16) return launch_bwd<__nv_bfloat16>(p, s);
   if (dtype == B200S_FP16) return launch_bwd<__half>(p, s);
   return launch_bwd<float>(p, s);
+}
+
+extern "C" {
+
+int b200s_token_logprobs(int64_t rows, int64_t vocab, int dtype, const void* logits, int64_t ld, const int64_t* targets,
+                         int64_t ignore_index, float* logprob, float* lse, float* entropy, int top_k, int64_t* top_ids,
+                         float* top_logprobs, void* stream) {
+  return logprobs_forward(rows, vocab, dtype, logits, ld, targets, ignore_index, logprob, lse, nullptr, entropy, top_k, top_ids,
+                          top_logprobs, stream);
+}
+
+int b200s_token_logprobs_stats(int64_t rows, int64_t vocab, int dtype, const void* logits, int64_t ld, const int64_t* targets,
+                               int64_t ignore_index, float* logprob, float* stats, float* entropy, int top_k, int64_t* top_ids,
+                               float* top_logprobs, void* stream) {
+  return logprobs_forward(rows, vocab, dtype, logits, ld, targets, ignore_index, logprob, nullptr, stats, entropy, top_k, top_ids,
+                          top_logprobs, stream);
+}
+
+int b200s_token_logprobs_backward(int64_t rows, int64_t vocab, int64_t width, int dtype, const void* logits, int64_t ld,
+                                  const int64_t* targets, int64_t ignore_index, const float* lse, const float* entropy,
+                                  const float* dlogprob, const float* dentropy, void* dlogits, int64_t ldd,
+                                  void* stream) {
+  return logprobs_backward(rows, vocab, width, dtype, logits, ld, targets, ignore_index, lse, nullptr, entropy, dlogprob, dentropy,
+                           dlogits, ldd, stream);
+}
+
+int b200s_token_logprobs_backward_stats(int64_t rows, int64_t vocab, int64_t width, int dtype, const void* logits, int64_t ld,
+                                        const int64_t* targets, int64_t ignore_index, const float* stats, const float* entropy,
+                                        const float* dlogprob, const float* dentropy, void* dlogits, int64_t ldd,
+                                        void* stream) {
+  return logprobs_backward(rows, vocab, width, dtype, logits, ld, targets, ignore_index, nullptr, stats, entropy, dlogprob, dentropy,
+                           dlogits, ldd, stream);
 }
 
 }  // extern "C"

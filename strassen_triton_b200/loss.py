@@ -2,7 +2,8 @@
 likely alternatives), and the mean loss `cross_entropy` built on it.
 
 One pass over the logits with a running maximum gives the log-sum-exp and the entropy of a row in fp32;
-the backward pass reads the logits once more and writes their gradient. No matrix of probabilities and
+the backward pass takes the maximum and the log of the sum apart (as one value they would be good to |lse| 2^-24
+only), reads the logits once more and writes their gradient. No matrix of probabilities and
 no fp32 copy of the logits exists at any time (the reference's training scripts call
 F.cross_entropy on logits.float(), which makes both).
 """
@@ -24,28 +25,30 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: Optional[Tensor]   # their log probabilities (fp32)
 
 
-def _forward(logits, targets, vocab, ignore_index, entropy, top_k, lse):
+def _forward(logits, targets, vocab, ignore_index, entropy, top_k, stats):
+    """(logprob, statistics, entropy, ids, their log probabilities): per row the maximum and the log of the sum, for the
+    backward pass, or None without ``stats``."""
     xr, rows, ld = rows_of(logits)
     t = targets.contiguous()
     lp = torch.empty_like(t, dtype=torch.float32)
     ent = torch.empty_like(lp) if entropy else None
-    ls = torch.empty_like(lp) if lse else None
+    st = lp.new_empty(t.shape + (2,)) if stats else None
     ids = t.new_empty(t.shape + (top_k,)) if top_k else None
     top = torch.empty_like(ids, dtype=torch.float32) if top_k else None
-    call(logits.device, _lib.load().b200s_token_logprobs, rows, vocab, dtype_code(logits, "logits"), xr.data_ptr(), ld, t.data_ptr(),
-         ignore_index, lp.data_ptr(), ptr(ls), ptr(ent), top_k, ptr(ids), ptr(top))
-    return lp, ls, ent, ids, top
+    call(logits.device, _lib.load().b200s_token_logprobs_stats, rows, vocab, dtype_code(logits, "logits"), xr.data_ptr(), ld, t.data_ptr(),
+         ignore_index, lp.data_ptr(), ptr(st), ptr(ent), top_k, ptr(ids), ptr(top))
+    return lp, st, ent, ids, top
 
 
-def _backward(logits, targets, vocab, ignore_index, lse, entropy, dlogprob, dentropy):
+def _backward(logits, targets, vocab, ignore_index, stats, entropy, dlogprob, dentropy):
     xr, rows, ld = rows_of(logits)
     t = targets.contiguous()
     dl, de = (g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.to(torch.float32).contiguous()
               for g in (dlogprob, dentropy))
     out = empty_as(logits)
     width = logits.shape[-1]
-    call(logits.device, _lib.load().b200s_token_logprobs_backward, rows, vocab, width, dtype_code(logits, "logits"),
-         xr.data_ptr(), ld, t.data_ptr(), ignore_index, lse.data_ptr(), ptr(entropy if de is not None else None),
+    call(logits.device, _lib.load().b200s_token_logprobs_backward_stats, rows, vocab, width, dtype_code(logits, "logits"),
+         xr.data_ptr(), ld, t.data_ptr(), ignore_index, stats.data_ptr(), ptr(entropy if de is not None else None),
          ptr(dl), ptr(de), out.data_ptr(), width)
     return out
 
@@ -53,9 +56,9 @@ def _backward(logits, targets, vocab, ignore_index, lse, entropy, dlogprob, dent
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, vocab, ignore_index, entropy, top_k):
-        lp, lse, ent, ids, top = _forward(logits, targets, vocab, ignore_index, entropy, top_k, True)
+        lp, st, ent, ids, top = _forward(logits, targets, vocab, ignore_index, entropy, top_k, True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, targets, lse, ent)
+        ctx.save_for_backward(logits, targets, st, ent)
         ctx.cfg = (vocab, ignore_index)
         if top_k:
             ctx.mark_non_differentiable(ids, top)
@@ -64,19 +67,19 @@ class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     @once
     def backward(ctx, dlp, dent, _dids, _dtop):
-        logits, targets, lse, ent = ctx.saved_tensors
+        logits, targets, st, ent = ctx.saved_tensors
         if dlp is None and dent is None:
             return None, None, None, None, None, None
-        return _backward(logits, targets, *ctx.cfg, lse, ent, dlp, dent), None, None, None, None, None
+        return _backward(logits, targets, *ctx.cfg, st, ent, dlp, dent), None, None, None, None, None
 
 
 # Opaque operators for traced graphs (torch.compile). Outputs that were not asked for are empty.
 @torch.library.custom_op("b200s::token_logprobs", mutates_args=())
 def _logprobs_op(logits: Tensor, targets: Tensor, vocab: int, ignore_index: int, entropy: bool,
                  top_k: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    lp, lse, ent, ids, top = _forward(logits, targets, vocab, ignore_index, entropy, top_k, True)
+    lp, st, ent, ids, top = _forward(logits, targets, vocab, ignore_index, entropy, top_k, True)
     e = lambda dt: torch.empty(0, dtype=dt, device=logits.device)  # noqa: E731
-    return (lp, lse, e(torch.float32) if ent is None else ent, e(torch.int64) if ids is None else ids,
+    return (lp, st, e(torch.float32) if ent is None else ent, e(torch.int64) if ids is None else ids,
             e(torch.float32) if top is None else top)
 
 
@@ -85,34 +88,34 @@ def _(logits, targets, vocab, ignore_index, entropy, top_k):
     f = lambda *s: logits.new_empty(s, dtype=torch.float32)  # noqa: E731
     shape = tuple(targets.shape)
     tops = shape + (top_k,) if top_k else (0,)
-    return (f(*shape), f(*shape), f(*(shape if entropy else (0,))), logits.new_empty(tops, dtype=torch.int64), f(*tops))
+    return (f(*shape), f(*shape, 2), f(*(shape if entropy else (0,))), logits.new_empty(tops, dtype=torch.int64), f(*tops))
 
 
 @torch.library.custom_op("b200s::token_logprobs_backward", mutates_args=())
-def _logprobs_backward_op(logits: Tensor, targets: Tensor, vocab: int, ignore_index: int, lse: Tensor,
+def _logprobs_backward_op(logits: Tensor, targets: Tensor, vocab: int, ignore_index: int, stats: Tensor,
                           entropy: Optional[Tensor], dlogprob: Optional[Tensor], dentropy: Optional[Tensor]) -> Tensor:
-    return _backward(logits, targets, vocab, ignore_index, lse, entropy, dlogprob, dentropy)
+    return _backward(logits, targets, vocab, ignore_index, stats, entropy, dlogprob, dentropy)
 
 
 @_logprobs_backward_op.register_fake
-def _(logits, targets, vocab, ignore_index, lse, entropy, dlogprob, dentropy):
+def _(logits, targets, vocab, ignore_index, stats, entropy, dlogprob, dentropy):
     return logits.new_empty(logits.shape)
 
 
 def _op_setup(ctx, inputs, output):
     logits, targets, vocab, ignore_index, entropy, _ = inputs
-    _, lse, ent, _, _ = output
-    ctx.save_for_backward(logits, targets, lse, ent)
+    _, st, ent, _, _ = output
+    ctx.save_for_backward(logits, targets, st, ent)
     ctx.cfg = (vocab, ignore_index, entropy)
     ctx.set_materialize_grads(False)
 
 
-def _op_backward(ctx, dlp, _dlse, dent, _dids, _dtop):
-    logits, targets, lse, ent = ctx.saved_tensors
+def _op_backward(ctx, dlp, _dstats, dent, _dids, _dtop):
+    logits, targets, st, ent = ctx.saved_tensors
     vocab, ignore_index, has_ent = ctx.cfg
     if dlp is None and (dent is None or not has_ent):
         return None, None, None, None, None, None
-    g = _logprobs_backward_op(logits, targets, vocab, ignore_index, lse, ent if has_ent else None, dlp,
+    g = _logprobs_backward_op(logits, targets, vocab, ignore_index, st, ent if has_ent else None, dlp,
                               dent if has_ent else None)
     return g, None, None, None, None, None
 
