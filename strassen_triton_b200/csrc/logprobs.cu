@@ -439,7 +439,8 @@ __global__ void __launch_bounds__(kThreads, 5) logprob_fwd_kernel(const LogprobF
             p.stats[r] = lse;
         }
         if (ENT) p.entropy[r] = lse == kNegInf ? 0.f : logs - a.u / a.s;
-        row_result = make_float2(lse == kNegInf ? kNegInf : a.m, logs);
+        // the alternatives' log probabilities are (x - a.m) - logs; -inf in an empty row, NaN in one whose lse is
+        row_result = make_float2(a.m == kNegInf ? lse : a.m, logs);
       }
       if constexpr (TOP) {
         __syncthreads();

@@ -1,0 +1,28 @@
+"""Rows of logits and targets at the edge of what token log probabilities are defined for."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.fixture(scope="module")
+def b200s(built_library):
+    if not torch.cuda.is_available():
+        pytest.fail("these tests need a CUDA device")
+    import strassen_triton_b200
+
+    return strassen_triton_b200
+
+
+@pytest.mark.parametrize("vocab,rows", [(3, 1), (500, 2), (9001, 4), (9001, 400)])
+@pytest.mark.parametrize("others", [-INF, 0.5, INF])
+def test_a_nan_makes_the_alternatives_nan(b200s, vocab, rows, others):
+    """Whatever the row's other logits are; the NaN itself is the first of them, then the lowest ids of the others."""
+    x = torch.full((rows, vocab), others, device="cuda")
+    x[:, 1] = NAN
+    t = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    r = b200s.token_logprobs(x, t, entropy=True, top_k=2)
+    assert torch.isnan(r.logprob).all() and torch.isnan(r.entropy).all() and torch.isnan(r.top_logprobs).all()
+    assert torch.equal(r.top_ids, torch.tensor([1, 0], device="cuda").expand(rows, 2))
