@@ -499,9 +499,10 @@ __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobBwd 
   float gl = p.dlogprob && !ignored ? p.dlogprob[r] : 0.f;
   float ge = ENT ? p.dentropy[r] : 0.f;
   const float h = ENT ? p.entropy[r] - st.y : 0.f;      // log p_i + entropy = (x_i - m) + h
-  if (!ignored && (t < 0 || t >= p.vocab)) gl = nan_f();
+  const bool outside = !ignored && (t < 0 || t >= p.vocab);
+  if (outside) gl = nan_f();
   // an ignored row stays zero whatever its logits hold
-  const bool none = lse == kNegInf || (gl == 0.f && ge == 0.f && (ignored || lse == lse));
+  const bool none = (lse == kNegInf && !outside) || (gl == 0.f && ge == 0.f && (ignored || lse == lse));
   const int limit = none ? 0 : p.vocab;
   const int target = t >= 0 && t < limit && !ignored ? static_cast<int>(t) : -1;
   const float gt = gl;

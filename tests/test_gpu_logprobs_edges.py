@@ -26,3 +26,15 @@ def test_a_nan_makes_the_alternatives_nan(b200s, vocab, rows, others):
     r = b200s.token_logprobs(x, t, entropy=True, top_k=2)
     assert torch.isnan(r.logprob).all() and torch.isnan(r.entropy).all() and torch.isnan(r.top_logprobs).all()
     assert torch.equal(r.top_ids, torch.tensor([1, 0], device="cuda").expand(rows, 2))
+
+
+@pytest.mark.parametrize("vocab,rows", [(3, 2), (500, 4), (9001, 3)])
+def test_a_target_out_of_range_makes_the_gradient_nan_in_an_empty_row_too(b200s, vocab, rows):
+    """Its log probability is NaN there as in any other row; a forbidden target's row has no gradient."""
+    x = torch.full((rows, vocab), -INF, device="cuda", requires_grad=True)
+    t = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    t[0] = vocab
+    lp = b200s.token_logprobs(x, t).logprob
+    assert torch.isnan(lp[0]) and (lp[1:] == -INF).all()
+    d, = torch.autograd.grad(lp, x, torch.ones_like(lp))
+    assert torch.isnan(d[0]).all() and not d[1:].any()
