@@ -458,7 +458,7 @@ int b200s_token_logprobs(int64_t rows, int64_t vocab, int dtype, const void* log
  * dlogits (rows x width of dtype, columns from vocab on zero) from the gradients of the log
  * probabilities and of the entropies (each may be NULL: zero), with lse and entropy as the forward call
  * wrote them (entropy is needed with dentropy only). Rows that were ignored and have no entropy gradient,
- * and rows without a finite logit, get zeros, rows whose target is out of range NaN. dlogits may be the logits themselves (same ld).
+ * and rows without a finite logit, get zeros, with dlogprob rows whose target is out of range NaN. dlogits may be the logits themselves (same ld).
  */
 int b200s_token_logprobs_backward(int64_t rows, int64_t vocab, int64_t width, int dtype, const void* logits_device,
                                   int64_t ld, const int64_t* targets_device, int64_t ignore_index,

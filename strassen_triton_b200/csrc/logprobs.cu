@@ -499,12 +499,12 @@ __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobBwd 
   float gl = p.dlogprob && !ignored ? p.dlogprob[r] : 0.f;
   float ge = ENT ? p.dentropy[r] : 0.f;
   const float h = ENT ? p.entropy[r] - st.y : 0.f;      // log p_i + entropy = (x_i - m) + h
-  const bool outside = !ignored && (t < 0 || t >= p.vocab);
+  const bool outside = p.dlogprob && !ignored && (t < 0 || t >= p.vocab);      // the entropy does not see the target
   if (outside) gl = nan_f();
   // an ignored row stays zero whatever its logits hold
   const bool none = (lse == kNegInf && !outside) || (gl == 0.f && ge == 0.f && (ignored || lse == lse));
   const int limit = none ? 0 : p.vocab;
-  const int target = t >= 0 && t < limit && !ignored ? static_cast<int>(t) : -1;
+  const int target = p.dlogprob && t >= 0 && t < limit && !ignored ? static_cast<int>(t) : -1;
   const float gt = gl;
   gl *= expf(-st.y);
   if constexpr (ENT) ge *= expf(-st.y);
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobBwd 
     }
   }
   const int at = target - sp.head;
-  if (at >= 0 && target < sp.tail() && (at / V - first) % step == 0) d[target] = from_f<T>(value(to_f(at_target), p.dlogprob ? p.dlogprob[r] : 0.f));
+  if (at >= 0 && target < sp.tail() && (at / V - first) % step == 0) d[target] = from_f<T>(value(to_f(at_target), p.dlogprob[r]));
 }
 
 int check_logits(int64_t rows, int64_t vocab, int dtype) {

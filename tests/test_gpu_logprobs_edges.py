@@ -38,3 +38,17 @@ def test_a_target_out_of_range_makes_the_gradient_nan_in_an_empty_row_too(b200s,
     assert torch.isnan(lp[0]) and (lp[1:] == -INF).all()
     d, = torch.autograd.grad(lp, x, torch.ones_like(lp))
     assert torch.isnan(d[0]).all() and not d[1:].any()
+
+
+@pytest.mark.parametrize("vocab,rows", [(50, 2), (9001, 3), (2000, 300)])
+def test_the_entropy_does_not_see_the_target(b200s, vocab, rows):
+    """An entropy alone has the same gradient for every target: in range, ignored or out of range."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(rows, vocab, generator=g, device="cuda").requires_grad_(True)
+    got = []
+    for target in (0, -100, -1, vocab):
+        t = torch.full((rows,), target, device="cuda")
+        r = b200s.token_logprobs(x, t, entropy=True)
+        got.append(torch.autograd.grad(r.entropy.sum(), x)[0])
+    assert torch.isfinite(got[0]).all() and got[0].any()
+    assert all(torch.equal(got[0], d) for d in got[1:])
