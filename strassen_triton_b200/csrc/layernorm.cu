@@ -757,17 +757,19 @@ norm_bwd_ring_kernel(const NormBwd p, int stages, uint32_t* status) {
 
 // Rows on their way per block: what fits 200 KB of an SM's shared memory shared by `per_sm` blocks, at
 // most 8; fewer than two are not worth it (the register forms then keep one row ahead themselves).
+constexpr int kRingBudget = 200 * 1024;
 int ring_stages(uint32_t stage_bytes, int per_sm) {
-  const int n = static_cast<int>(200 * 1024 / per_sm / stage_bytes);
+  const int n = static_cast<int>(kRingBudget / per_sm / stage_bytes);
   return n > 8 ? 8 : n;
 }
 
 template <class K>
-int allow_smem(K kernel, size_t bytes) {
-  // what a launch gets unasked is 48 KB less the kernel's static shared memory (a few hundred bytes);
-  // per device and kernel once would do; the call is cheap and has no state to go wrong
+int allow_smem(K kernel, size_t bytes, int per_sm) {
+  // What a launch gets unasked is 48 KB less the kernel's static shared memory (a few hundred bytes). The limit
+  // belongs to the kernel on a device, which rows of many lengths share: it is set to the most any of them asks for,
+  // so that a call never lowers it between another thread's setting and its launch.
   if (bytes <= 47 * 1024) return B200S_OK;
-  B200S_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+  B200S_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 + kRingBudget / per_sm));
   return B200S_OK;
 }
 
@@ -912,7 +914,7 @@ int b200s_layer_norm(int64_t rows, int64_t d, int dtype, int param_dtype, float 
           const int stages = ring_stages(bytes, per_sm);
           if (stages >= 2 && rows > 148 * per_sm) {
             auto kernel = norm_fwd_ring_kernel<typename F::type, typename F::param, F::vec, F::nv, F::threads>;
-            int rc2 = allow_smem(kernel, 128 + static_cast<size_t>(stages) * bytes);
+            int rc2 = allow_smem(kernel, 128 + static_cast<size_t>(stages) * bytes, per_sm);
             if (rc2) return rc2;
             kernel<<<148 * per_sm, form.threads, 128 + static_cast<size_t>(stages) * bytes, s>>>(p, stages, device_status_words());
             B200S_CUDA_OK(cudaGetLastError());
@@ -992,7 +994,7 @@ int b200s_layer_norm_backward(int64_t rows, int64_t d, int dtype, int param_dtyp
           const int stages = ring_stages(bytes, blocks_per_sm(form));
           if (stages >= 2 && rows > slices) {
             auto kernel = norm_bwd_ring_kernel<T, typename F::param, F::vec, F::nv, F::threads>;
-            int rc3 = allow_smem(kernel, 128 + static_cast<size_t>(stages) * bytes);
+            int rc3 = allow_smem(kernel, 128 + static_cast<size_t>(stages) * bytes, blocks_per_sm(form));
             if (rc3) return rc3;
             kernel<<<slices, form.threads, 128 + static_cast<size_t>(stages) * bytes, s>>>(p, stages, device_status_words());
             B200S_CUDA_OK(cudaGetLastError());
