@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -90,6 +91,15 @@ def once(backward):
         return slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
+
+
+def refuse_tangents(*tensors) -> None:
+    """The operators have no forward-mode derivative: a dual tensor's would be lost in silence."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("this operator has no forward-mode derivative (got a dual tensor)")
 
 
 def wants_grad(*tensors) -> bool:

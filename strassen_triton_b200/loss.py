@@ -15,7 +15,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._call import call, dtype_code, empty_as, once, ptr, require_cuda, rows_of, wants_grad
+from ._call import call, dtype_code, empty_as, once, ptr, refuse_tangents, require_cuda, rows_of, wants_grad
 
 
 class TokenLogprobs(NamedTuple):
@@ -153,6 +153,7 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, vocab: Optional[int] = No
     if torch.compiler.is_compiling():
         lp, _, ent, ids, top = _logprobs_op(logits, targets, vocab, ignore_index, bool(entropy), top_k)
         return TokenLogprobs(lp, ent if entropy else None, ids if top_k else None, top if top_k else None)
+    refuse_tangents(logits)
     if wants_grad(logits):
         return TokenLogprobs(*_TokenLogprobsFn.apply(logits, targets, vocab, ignore_index, bool(entropy), top_k))
     lp, _, ent, ids, top = _forward(logits, targets, vocab, ignore_index, bool(entropy), top_k, False)

@@ -16,7 +16,8 @@ import torch.nn as nn
 from torch import Tensor
 
 from . import _lib
-from ._call import DTYPE, call, dtype_code, empty, empty_as, empty_rows, once, ptr, require_cuda, rows_of, wants_grad
+from ._call import (DTYPE, call, dtype_code, empty, empty_as, empty_rows, once, ptr, refuse_tangents, require_cuda, rows_of,
+                    wants_grad)
 
 
 def _check(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]) -> None:
@@ -158,6 +159,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     _check(x, weight, bias)
     if torch.compiler.is_compiling():
         return _layer_norm_op(x, weight, bias, float(eps))[0]
+    refuse_tangents(x, weight, bias)
     if wants_grad(x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, float(eps))
     return _forward(x, weight, bias, float(eps), False)[0]

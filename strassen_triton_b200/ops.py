@@ -286,12 +286,16 @@ _linear_op.register_autograd(_linear_backward, setup_context=_linear_setup)
 def linear_autograd(X, W, bias, algo="auto", depth=-1):
     """Differentiable X @ W + bias (X 2-D, W = weight.T as a view), the bias fused into the epilogue."""
     _require_cuda(X, W, bias)
+    if not torch.compiler.is_compiling():
+        _call.refuse_tangents(X, W, bias)
     return _linear_op(X, W, bias, algo, int(depth))
 
 
 def matmul_autograd(X, W, algo="auto", depth=-1, prod_dtype=None):
     """Differentiable X @ W (2-D or batched 3-D operands); traceable by torch.compile."""
     _require_cuda(X, W)
+    if not torch.compiler.is_compiling():
+        _call.refuse_tangents(X, W)
     return _matmul_op(X, W, algo, int(depth), _DT_NAME[prod_dtype])
 
 
@@ -575,6 +579,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     four; for the backward pass the pre-activation is kept in x's type. ``algo``, ``depth`` and ``precision`` choose
     the products, forward and backward, as in `matmul`."""
     _call.require_cuda(x, weight, bias, residual)
+    if not torch.compiler.is_compiling():
+        _call.refuse_tangents(x, weight, bias, residual)
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
