@@ -34,6 +34,13 @@ using row::to_f;
 
 constexpr int kThreads = 256;
 
+// s / d with the rounding of a division (1 / d alone is rounded already, and a row of one value would differ from its
+// mean): the quotient's remainder, formed exactly by the fused operation, corrects it.
+__device__ __forceinline__ float mean_of(float s, float inv_d, float d) {
+  const float q = s * inv_d;
+  return fmaf(fmaf(-q, d, s), inv_d, q);
+}
+
 struct NormFwd {
   const void* x;
   const void* w;
@@ -55,7 +62,7 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_any_kernel(const NormFwd p)
     T* y = static_cast<T*>(p.y) + r * p.ldy;
     float s = 0.f;
     for (int64_t c = threadIdx.x; c < p.d; c += kThreads) s += to_f(x[c]);
-    const float mu = row::block_sum(s, slots) * inv_d;
+    const float mu = mean_of(row::block_sum(s, slots), inv_d, static_cast<float>(p.d));
     float q = 0.f;
     for (int64_t c = threadIdx.x; c < p.d; c += kThreads) {
       const float t = to_f(x[c]) - mu;
@@ -300,7 +307,7 @@ __global__ void __launch_bounds__(TH == 32 ? 32 * kWarpRows : TH) norm_fwd_kerne
         s = add_(s, x[i][k]);
       }
     if (r + step < p.rows) fetch(r + step);
-    const float mu = row_sum<TH>(hsum(s), slots, flip) * inv_d;
+    const float mu = mean_of(row_sum<TH>(hsum(s), slots, flip), inv_d, static_cast<float>(d));
     const F shift = U::all(-mu);
     F q = U::all(0.f);
 #pragma unroll
@@ -588,7 +595,7 @@ norm_fwd_ring_kernel(const NormFwd p, int stages, uint32_t* status) {
         }
       }
     }
-    const float mu = row_sum<TH, true>(hsum(s), slots, flip, &ok) * inv_d;
+    const float mu = mean_of(row_sum<TH, true>(hsum(s), slots, flip, &ok), inv_d, static_cast<float>(d));
     if (!ok) {
       const int64_t left = (p.rows - r + step - 1) / step;
       give_up(ring, at, static_cast<int>(left < stages ? left : stages), status);
