@@ -7,7 +7,13 @@
 // A dense product of 16-bit operands and results runs its epilogue inside the product's kernel
 // (linear_sm100.cu). For every other product b200s_matmul takes (fp32, Strassen), and where K is cut into
 // parts, fp32 products go to scratch and one pass here adds them up, adds the bias, applies the activation,
-// adds the residual and rounds once. The pre-activation z the backward pass needs is stored in the type of C.
+// adds the residual and rounds once.
+//
+// Two roundings of the backward pass of 16-bit layers are choices. The pre-activation z it needs is stored in the type
+// of C: in fp32 it would double the largest tensor kept between the passes (its rounding adds 6e-4 of the gradients'
+// norm in bf16, 6e-5 in fp16). dz goes to the products of dx and dw in 16 bits, as the tensor cores take both operands
+// (1.6e-3, 2e-4); dbias is summed before that rounding. Together dx and dw have 1.45 times the error of gradients
+// that are rounded at the end only (2.4e-3 against 1.7e-3 in bf16, 3.0e-4 against 2.1e-4 in fp16).
 
 #include <cuda_runtime.h>
 

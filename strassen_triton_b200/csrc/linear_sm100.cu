@@ -10,11 +10,13 @@
 //   skinny_kernel   up to 16 rows of A (tokens being generated) against K-major weights: bound by reading the
 //                   weights once, with mma.sync fed straight from global memory in registers.
 //
-// What bounds linear_kernel: L2 reads of operand tiles. A 256 x 256 pair reads 64 KB per 64 of K, and with all
-// SMs loading the steps come 0.39 .. 0.48 us apart, about 12 TB/s, where the tensor cores need 0.27. (A library
-// product that shares tiles between clusters by multicast, which this package does without, takes 337 us for
-// 8192 x 4096 x 8192 where this kernel takes 374 and with GELU and bias 389.) With K below about 1000 the epilogue's
-// arithmetic adds to it: 8192 x 768 -> 2304 takes 28 us plain, 37 with GELU and bias, 41 with z stored too.
+// What bounds linear_kernel. Products of many tiles: L2 reads of operand tiles. A 256 x 256 pair reads 64 KB per 64
+// of K, and with all SMs loading the steps come 0.39 .. 0.48 us apart, about 12 TB/s, where the tensor cores need
+// 0.27 (8192 x 4096 x 8192: 374 us, with GELU and bias 389; the library product 337). With K below about 1000 the
+// epilogue's arithmetic adds to it: 8192 x 768 -> 2304 takes 28 us plain, 37 with GELU and bias, 41 with z stored too.
+// Products of few tiles: the last round. The gradients of that layer are 96 tiles for 74 pairs, two rounds with 22
+// pairs at work in the second (dx, 37 us, tensor pipe at 54 %), and 27 tiles in two parts, 54 pairs at work, with
+// the pass over the partial products behind them (dw, 33 + 6 us).
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -83,9 +85,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
 }
 __device__ __forceinline__ float2 unpack2(uint32_t u, bool bf16) {
   return bf16 ? make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&u));
-}
-__device__ __forceinline__ float element(const void* p, int64_t i, bool bf16) {
-  return bf16 ? __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + i)) : __half2float(__ldg(static_cast<const __half*>(p) + i));
 }
 
 template <int ACT>
