@@ -202,6 +202,10 @@ def clip_grads_(grads: Iterable[Tensor], max_norm: float, *, out: Optional[Seque
                     dst.append(torch.empty(o.shape, dtype=o.dtype, device=dev))
                     back.append((o, dst[-1]))
             arr = _entries(src, dst)
+    if back:      # the kernels see copies of these, and no overlap
+        written = [(t.data_ptr(), t.shape, t.stride()) for t, _ in back if t.numel()]
+        if len(set(written)) < len(written):
+            raise ValueError("a tensor that is written appears twice in the list")
     lib = _lib.load()
     parts, n_parts = _sumsq(dev, arr, len(grads), group)
     norm = torch.empty_strided((), (), dtype=torch.float32, device=dev)
