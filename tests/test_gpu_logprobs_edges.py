@@ -52,3 +52,26 @@ def test_the_entropy_does_not_see_the_target(b200s, vocab, rows):
         got.append(torch.autograd.grad(r.entropy.sum(), x)[0])
     assert torch.isfinite(got[0]).all() and got[0].any()
     assert all(torch.equal(got[0], d) for d in got[1:])
+
+
+@pytest.mark.parametrize("rows,vocab,width", [(1, 50257, 50304), (3, 9001, 9001), (400, 1000, 1003)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_in_the_logits_own_memory(b200s, rows, vocab, width, dtype):
+    """The C entry may write the gradient over the logits: the same bits as into another buffer, wherever the target
+    lies (a row's head, body and tail, and every block that shares it)."""
+    from strassen_triton_b200 import _lib
+
+    lib, code = _lib.load(), {torch.bfloat16: _lib.BF16, torch.float32: _lib.FP32}[dtype]
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (torch.randn(rows, width, generator=g, device="cuda") * 3).to(dtype)
+    dlp, dent = (torch.randn(rows, generator=g, device="cuda") for _ in range(2))
+    lp, ent, st = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty(rows, 2, device="cuda")
+    s, p = torch.cuda.current_stream().cuda_stream, lambda a: a.data_ptr()
+    for first in (0, 1, 7, 8, 2047, 2048, vocab // 2, vocab - 3):
+        t = (torch.arange(rows, device="cuda") + first) % vocab
+        assert lib.b200s_token_logprobs_stats(rows, vocab, code, p(x), width, p(t), -100, p(lp), p(st), p(ent), 0, None, None, s) == 0
+        out, own = torch.empty_like(x), x.clone()
+        for src, dst in ((x, out), (own, own)):
+            assert lib.b200s_token_logprobs_backward_stats(rows, vocab, width, code, p(src), width, p(t), -100, p(st), p(ent),
+                                                           p(dlp), p(dent), p(dst), width, s) == 0
+        assert torch.equal(out, own)
