@@ -552,7 +552,7 @@ using namespace b200s;
 
 extern "C" {
 
-int b200s_version(void) { return 200; }
+int b200s_version(void) { return 201; }
 
 const char* b200s_status_string(int status) {
   switch (status) {

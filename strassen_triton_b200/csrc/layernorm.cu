@@ -17,7 +17,7 @@
 // take the looping kernels, which read a row again (from L1 / L2) instead of keeping it.
 //
 // Measured: 16381 x 4096 fp16 with fp32 parameters 48 us forward (5.6 TB/s) and 76 + 4 us backward (5.3 TB/s);
-// 8192 x 768 bf16, resident in L2, 6.4 us and 12.4 + 4 us, where latency counts: a warp has one to five rows.
+// 8192 x 768 bf16, resident in L2, 6.6 us and 16 us together, where latency counts: a warp has one to five rows.
 
 #include <cuda_runtime.h>
 

@@ -13,10 +13,11 @@
 // What bounds linear_kernel. Products of many tiles: L2 reads of operand tiles. A 256 x 256 pair reads 64 KB per 64
 // of K, and with all SMs loading the steps come 0.39 .. 0.48 us apart, about 12 TB/s, where the tensor cores need
 // 0.27 (8192 x 4096 x 8192: 374 us, with GELU and bias 389; the library product 337). With K below about 1000 the
-// epilogue's arithmetic adds to it: 8192 x 768 -> 2304 takes 28 us plain, 37 with GELU and bias, 41 with z stored too.
+// epilogue's arithmetic adds to it: 8192 x 768 -> 2304 takes 27 us plain, 36 with GELU and bias, 40 with z stored too.
 // Products of few tiles: the last round. The gradients of that layer are 96 tiles for 74 pairs, two rounds with 22
-// pairs at work in the second (dx, 37 us, tensor pipe at 54 %), and 27 tiles in two parts, 54 pairs at work, with
-// the pass over the partial products behind them (dw, 33 + 6 us).
+// pairs at work in the second (dx, 32 us; with a cold L2 38, tensor pipe at 55 %), and 27 tiles in two parts, 54
+// pairs at work, with the pass over the partial products behind them (dw, 33 us together). The library products take
+// 23 (plain), 22 and 23.
 
 #include <cuda.h>
 #include <cuda_bf16.h>

@@ -577,7 +577,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     All of one type (bias is converted); rows may be strided and of any length (operand rows that are not whole
     16-byte vectors are copied). Everything after the product is fp32 and rounded once. Differentiable once in all
     four; for the backward pass the pre-activation is kept in x's type. ``algo``, ``depth`` and ``precision`` choose
-    the products, forward and backward, as in `matmul`."""
+    the products, forward and backward, as in `matmul`. Inside torch.compile the layer always keeps the
+    pre-activation and its backward pass computes the gradients of x, weight and bias whether needed or not."""
     _call.require_cuda(x, weight, bias, residual)
     if not torch.compiler.is_compiling():
         _call.refuse_tangents(x, weight, bias, residual)
